@@ -915,6 +915,62 @@ LH_API int lh_moe_vector_routed_up_into(lh_batch* batch, const lh_buffer* input,
 LH_API int lh_moe_vector_down_into(lh_batch* batch, const lh_buffer* hidden, const lh_buffer* logits, const lh_buffer* down,
                                    lh_buffer* residual, uint32_t experts, uint32_t top, uint32_t width, uint32_t ff);
 
+/* Rotary positions.  Of every head of `dim` values the columns first .. first + rot - 1 are turned in pairs by the position of their
+ * row: (a, b) becomes amplitude * (a cos - b sin, b cos + a sin) of the angle position * frequencies[i], f32 [rot / 2]; the other
+ * columns are copied.  Angles are formed and reduced in 64 bits, results rounded once.
+ *   LH_ROTARY_PAIRS    pair i is columns 2 i and 2 i + 1 of the turned part
+ *   LH_ROTARY_HALVES   pair i is columns i and i + rot / 2
+ *   frequencies  host side, no GPU work: base^(-2 i / rot); LINEAR: all of them divided by `factor`; BY_PARTS: those that make at least
+ *                `fast` turns in `original` positions stay, those that make at most `slow` are divided, the ones between shade over
+ *                (NTK by parts, "YaRN": Peng et al., 2023), and *amplitude is 0.1 ln(factor) + 1 (else 1)
+ *   rows         input and output rows of [heads, dim], input_ld and output_ld values apart; LH_F16, LH_BF16 or LH_F32; positions u32
+ *                [rows] in device memory.  Output may be the input (same buffer, same distance) and may not overlap it otherwise. */
+#define LH_ROTARY_PAIRS 0
+#define LH_ROTARY_HALVES 1
+#define LH_ROTARY_PLAIN 0
+#define LH_ROTARY_LINEAR 1
+#define LH_ROTARY_BY_PARTS 2
+LH_API int lh_rotary_frequencies(uint32_t rot, float base, uint32_t scaling, float factor, float original, float fast, float slow,
+                                 float* frequencies, float* amplitude);
+LH_API int lh_rotary_rows_into(lh_batch* batch, const lh_buffer* input, lh_buffer* output, int dtype, const lh_buffer* positions,
+                               const lh_buffer* frequencies, float amplitude, uint32_t rows, uint32_t heads, uint32_t dim,
+                               uint32_t rot, uint32_t first, uint32_t pairing, uint32_t input_ld, uint32_t output_ld);
+
+/* Caches in pages: the keys and the values of many sequences in one pool each, [pages][kv_heads][page][lh_paged_padded_dim(dim)] of
+ * `dtype` (LH_F16, LH_BF16 or LH_F32), `page` positions to a page (a power of two, 16 .. 1024), heads of up to 256 dimensions.  A step's
+ * rows are those of its sequences one after the other.  In device memory, u32:
+ *   table    [sequences, table_ld]: the page of every `page` positions of a sequence.  Sequences may share pages that none of them
+ *            appends to.
+ *   starts   [sequences + 1]: rows starts[s] .. starts[s + 1] - 1 are of sequence s (none, where it takes no part)
+ *   lengths  [sequences]: positions of a sequence with its rows in; its last row stands at lengths[s] - 1.  Rows before position 0,
+ *            where a sequence has more rows than positions, stand nowhere.
+ * What a table says of pages that the pool does not have, and positions that the table does not reach, are dropped when written and not
+ * seen when read; rows of no sequence are left as they were, and so are those of one that ends behind `rows`.
+ *   append     k and v rows [kv_heads, dim], k_ld and v_ld values apart, go to their pages, k turned as in lh_rotary_rows_into; the
+ *              columns behind dim become zero.  q (may be null, with heads 0) is turned by the same positions into q_output, which may be
+ *              q (a row that stands nowhere is left out).  frequencies may be null with rot 0: nothing turns.  No two sequences append to
+ *              one slot.
+ *   attention  a row sees the positions up to its own, with `window` > 0 the last `window` of them; query heads share kv heads in equal
+ *              groups.  out = softmax average with `scale`; sink f32 [heads] (may be null): exp(sink) is one more term of the denominator.
+ *              A row that sees nothing becomes zero.  max_rows bounds a sequence's rows and max_length the lengths: they size the launch (a
+ *              recorded batch gives the largest it will be replayed with); rows and positions beyond them are left out.  `workspace` takes
+ *              lh_paged_attention_workspace_bytes (null where that is 0); its size goes by these arguments. */
+LH_API uint32_t lh_paged_padded_dim(uint32_t dim);
+LH_API int lh_paged_append_into(lh_batch* batch, const lh_buffer* k, const lh_buffer* v, int dtype, lh_buffer* keys, lh_buffer* values,
+                                const lh_buffer* table, const lh_buffer* starts, const lh_buffer* lengths, uint32_t rows,
+                                uint32_t sequences, uint32_t kv_heads, uint32_t dim, uint32_t pages, uint32_t page, uint32_t table_ld,
+                                uint32_t k_ld, uint32_t v_ld, const lh_buffer* frequencies, float amplitude, uint32_t rot,
+                                uint32_t first, uint32_t pairing, const lh_buffer* q, lh_buffer* q_output, uint32_t heads,
+                                uint32_t q_ld, uint32_t q_output_ld);
+LH_API size_t lh_paged_attention_workspace_bytes(uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length,
+                                                 uint32_t heads, uint32_t kv_heads, uint32_t dim);
+LH_API int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer* keys, const lh_buffer* values,
+                                   lh_buffer* output, int dtype, const lh_buffer* table, const lh_buffer* starts,
+                                   const lh_buffer* lengths, uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length,
+                                   uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t pages, uint32_t page, uint32_t table_ld,
+                                   uint32_t q_ld, uint32_t output_ld, float scale, uint32_t window, const lh_buffer* sink,
+                                   lh_buffer* workspace);
+
 /* *position += by (u32); the index of the largest of each row of f32 logits (ties: the lower index); both, for one row */
 LH_API int lh_advance_position_into(lh_batch* batch, lh_buffer* position, uint32_t by);
 LH_API int lh_argmax_rows_f32_into(lh_batch* batch, const lh_buffer* logits, lh_buffer* index, uint32_t rows, uint32_t n);

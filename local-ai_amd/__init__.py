@@ -34,6 +34,10 @@ MULTIVEC_MAX_M = 16   # local-metal/src/kernels.rs:6362
 ACT_NONE, ACT_SILU, ACT_GELU_TANH, ACT_RELU_SQUARED, ACT_SIGMOID, ACT_SILU_PAIRS = range(6)
 ROWS, ROWS_AT_POSITION, BLOCKS_AT_POSITION, ROWS_F32 = range(4)
 
+# how a head's values pair up for rotary positions, and how their frequencies are scaled for long contexts
+ROTARY_PAIRS, ROTARY_HALVES = range(2)
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BY_PARTS = range(3)
+
 
 class Error(Exception):
     """Mirror of ``local_metal::Error`` (local-metal/src/error.rs:1-32)."""
@@ -99,11 +103,13 @@ def lib() -> C.CDLL:
         for name in ("lh_smallm_max_m", "lh_batchm_max_m", "lh_multivec_max_m", "lh_batch_dispatch_count",
                      "lh_flash_split_count", "lh_attention_padded_dim", "lh_attention_padded_vdim",
                      "lh_linear_attention_padded_dim", "lh_moe_plan_words", "lh_latent_padded_rank", "lh_latent_row",
-                     "lh_gated_vector_fits"):
+                     "lh_gated_vector_fits", "lh_paged_padded_dim"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = C.c_uint32
         _lib.lh_linear_attention_workspace_bytes.restype = C.c_size_t
         _lib.lh_selective_steps_bytes.restype = C.c_size_t
+        if hasattr(_lib, "lh_paged_attention_workspace_bytes"):
+            _lib.lh_paged_attention_workspace_bytes.restype = C.c_size_t
     return _lib
 
 
@@ -952,6 +958,44 @@ class Kernels:
                                               _u32(max_position), _u32(rows), _u32(heads), _u32(kv_heads), _u32(maps),
                                               _u32(dim), _u32(vdim), _u32(capacity), C.c_float(scale), C.c_float(lam),
                                               C.c_float(out_scale), C.c_float(eps), _opt(sink), _opt(gate)))
+
+    # -- rotary positions and caches in pages --
+    @staticmethod
+    def rotary_frequencies(rot, base, scaling=ROTARY_PLAIN, factor=1.0, original=0.0, fast=32.0, slow=1.0):
+        """(frequencies f32 [rot / 2], amplitude) of `rot` turned columns."""
+        f, amplitude = np.empty(max(int(rot) // 2, 1), np.float32), C.c_float()
+        _check(lib().lh_rotary_frequencies(_u32(rot), C.c_float(base), _u32(scaling), C.c_float(factor), C.c_float(original), C.c_float(fast),
+                                           C.c_float(slow), C.c_void_p(f.ctypes.data), C.byref(amplitude)))
+        return f, float(amplitude.value)
+
+    def rotary_rows_into(self, batch, input, output, dtype, positions, frequencies, amplitude, rows, heads, dim, rot, first, pairing,
+                         input_ld, output_ld):
+        _check(self._l.lh_rotary_rows_into(batch._h, input._h, output._h, C.c_int(dtype), positions._h, frequencies._h, C.c_float(amplitude),
+                                           _u32(rows), _u32(heads), _u32(dim), _u32(rot), _u32(first), _u32(pairing), _u32(input_ld),
+                                           _u32(output_ld)))
+
+    def paged_padded_dim(self, dim):
+        return int(self._l.lh_paged_padded_dim(_u32(dim)))
+
+    def paged_append_into(self, batch, k, v, dtype, keys, values, table, starts, lengths, rows, sequences, kv_heads, dim, pages, page,
+                          table_ld, k_ld, v_ld, frequencies=None, amplitude=1.0, rot=0, first=0, pairing=ROTARY_PAIRS, q=None,
+                          q_output=None, heads=0, q_ld=0, q_output_ld=0):
+        _check(self._l.lh_paged_append_into(batch._h, k._h, v._h, C.c_int(dtype), keys._h, values._h, table._h, starts._h, lengths._h,
+                                            _u32(rows), _u32(sequences), _u32(kv_heads), _u32(dim), _u32(pages), _u32(page),
+                                            _u32(table_ld), _u32(k_ld), _u32(v_ld), _opt(frequencies), C.c_float(amplitude), _u32(rot),
+                                            _u32(first), _u32(pairing), _opt(q), _opt(q_output), _u32(heads), _u32(q_ld),
+                                            _u32(q_output_ld)))
+
+    def paged_attention_workspace_bytes(self, rows, sequences, max_rows, max_length, heads, kv_heads, dim):
+        return int(self._l.lh_paged_attention_workspace_bytes(_u32(rows), _u32(sequences), _u32(max_rows), _u32(max_length), _u32(heads),
+                                                              _u32(kv_heads), _u32(dim)))
+
+    def paged_attention_into(self, batch, q, keys, values, output, dtype, table, starts, lengths, rows, sequences, max_rows, max_length,
+                             heads, kv_heads, dim, pages, page, table_ld, q_ld, output_ld, scale, window=0, sink=None, workspace=None):
+        _check(self._l.lh_paged_attention_into(batch._h, q._h, keys._h, values._h, output._h, C.c_int(dtype), table._h, starts._h,
+                                               lengths._h, _u32(rows), _u32(sequences), _u32(max_rows), _u32(max_length), _u32(heads),
+                                               _u32(kv_heads), _u32(dim), _u32(pages), _u32(page), _u32(table_ld), _u32(q_ld),
+                                               _u32(output_ld), C.c_float(scale), _u32(window), _opt(sink), _opt(workspace)))
 
     def linear_attention_padded_dim(self, dim):
         return int(self._l.lh_linear_attention_padded_dim(_u32(dim)))

@@ -1,0 +1,519 @@
+// Softmax attention of a step's rows over a paged cache: one token of a sequence, a chunk, a whole prompt, sequences of each kind in one
+// launch.
+//
+//   out = sum_j softmax_j(scale q . k_j [, sink]) v_j   over the positions j up to the row's own, the last `window` of them where there is one
+//
+// A tile is 16 packed rows (row of the sequence, head of the group) of one kv head; the tiles of all sequences are counted off from
+// `starts` by every wave.  Running maximum and sum in 32 bits, in powers of two.
+#include "paged.hpp"
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+namespace {
+
+typedef _Float16 lh_f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct PagedArgs {
+    const void *q, *keys, *values;
+    void* out;
+    const float* sink;         // [heads], may be null
+    float* partial;            // records [tile][kv head][split][16][D + 4]: unnormalised sums, maximum, sum of weights
+    PagedPlan plan;
+    uint64_t q_ld, out_ld;
+    uint32_t max_rows, heads, kv_heads, dim, window, capacity;     // capacity: positions from there on are not seen
+    uint32_t tiles, splits, chunk;                                 // chunk: steps of 32 positions that a split takes at least
+    uint32_t q_wide, out_wide;                                     // rows, heads and their ends at 16 bytes
+    float scale;
+};
+
+// A tile of a sequence: its rows row0 .. row0 + count - 1 of the packed ones.
+struct Tile {
+    int sequence;
+    uint32_t row0, count, first;    // first: the sequence's first row in q
+    int64_t begin;                  // position of the sequence's first row
+};
+// All lanes get the same; sequence -1 behind the last tile.
+template <uint32_t ROWS>
+__device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t t, uint32_t lane) {
+    const uint32_t R = a.heads / a.kv_heads;
+    Tile r{-1, 0, 0, 0, 0};
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 64) {
+        const uint32_t s = s0 + lane;
+        uint32_t first = 0, all = 0, tiles = 0;
+        if (s < a.plan.sequences) {
+            first = a.plan.starts[s];
+            const uint32_t end = a.plan.starts[s + 1];
+            if (end > first && end <= a.plan.rows) {
+                all = end - first;
+                tiles = (uint32_t)(((uint64_t)min(all, a.max_rows) * R + ROWS - 1) / ROWS);
+            }
+        }
+        uint32_t sum = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) { const uint32_t x = __shfl_up(sum, d); if (lane >= (uint32_t)d) sum += x; }
+        const uint64_t behind = __ballot(before + sum > t);
+        if (behind) {
+            const int at = __builtin_ctzll(behind);
+            const uint32_t n = __builtin_amdgcn_readlane(all, at), rows = min(n, a.max_rows) * R;
+            r.sequence = s0 + at;
+            r.first = __builtin_amdgcn_readlane(first, at);
+            const uint32_t in = t - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at));
+            r.row0 = in * ROWS;
+            r.count = min(ROWS, rows - r.row0);
+            r.begin = (int64_t)a.plan.lengths[r.sequence] - n;
+            return r;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return r;
+}
+
+// Positions lo .. hi - 1 are seen by a sequence's row `row`.
+struct Seen { uint32_t lo, hi; };
+__device__ __forceinline__ Seen seen_by(const PagedArgs& a, const Tile& t, uint32_t row) {
+    const int64_t p = t.begin + row, cap = a.capacity;
+    Seen s;
+    s.hi = (uint32_t)min(max(p + 1, (int64_t)0), cap);
+    s.lo = a.window ? (uint32_t)min(max(p + 1 - a.window, (int64_t)0), cap) : 0u;
+    return s;
+}
+
+// The part of a tile's positions that split z takes, in steps of 32; `used` splits have any.
+struct Part { uint32_t begin, end, used; };
+__device__ __forceinline__ Part part_of(const PagedArgs& a, uint32_t lo, uint32_t hi, uint32_t z) {
+    const uint32_t b0 = lo / 32, b1 = max((hi + 31) / 32, b0), n = b1 - b0;
+    const uint32_t used = min(max((n + a.chunk - 1) / a.chunk, 1u), a.splits), per = (n + used - 1) / used;
+    return Part{min(b0 + z * per, b1), min(b0 + (z + 1) * per, b1), used};
+}
+
+// A wave's view of its sequence's row of the table: 64 entries at a time, one a lane.
+struct Pages {
+    const uint32_t* row;
+    uint32_t held, entry;           // entries held .. held + 63
+    __device__ __forceinline__ void load(const PagedPlan& p, uint32_t from, uint32_t lane) {
+        held = from;
+        entry = from + lane < p.table_ld ? row[from + lane] : 0xFFFFFFFFu;
+    }
+    __device__ __forceinline__ uint32_t of(const PagedPlan& p, uint32_t block, uint32_t lane) {
+        if (block - held >= 64) load(p, block, lane);
+        return __builtin_amdgcn_readlane(entry, block - held);
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ lh_f32x4 product(u32x4 x, u32x4 y, lh_f32x4 c) {
+    if constexpr (DT == kF16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lh_f16x8, x), __builtin_bit_cast(lh_f16x8, y), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lh_bf16x8, x), __builtin_bit_cast(lh_bf16x8, y), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (DT == kF16) return (uint32_t)lh_f2h(a) | (uint32_t)lh_f2h(b) << 16;
+    else return lh_pack_bf(a, b);
+}
+template <int DT>
+__device__ __forceinline__ float low(uint32_t x) { return element_value<DT>((element_t<DT>)(x & 0xFFFFu)); }
+template <int DT>
+__device__ __forceinline__ float high(uint32_t x) { return element_value<DT>((element_t<DT>)(x >> 16)); }
+
+// N dwords from an address that is a multiple of their largest power of two
+template <int N>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&x)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) { const u32x4 v = *reinterpret_cast<const u32x4*>((const char*)p + 4 * i); x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w; }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) { const uint2 v = *reinterpret_cast<const uint2*>((const char*)p + 4 * i); x[i] = v.x; x[i + 1] = v.y; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const uint32_t*>((const char*)p + 4 * i);
+    }
+}
+
+// One packed row over steps begin .. end - 1, by one wave and value by value: what takes the place of the matrix instructions where a
+// result is not a number.  There a position that a row does not see has the weight 0, and 0 times an infinity or NaN that stands in it
+// is NaN; here it is left out.  Every lane gets the maximum (in powers of two) and the sum; sums[c] is of column lane + 64 c.
+template <int DT, int D>
+__device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint64_t q_at, uint32_t g, uint32_t lo, uint32_t hi, uint32_t begin, uint32_t end, uint32_t lane,
+                                                   float& m, float& l, float (&sums)[(D + 63) / 64]) {
+    typedef element_t<DT> B;
+    constexpr int N = (D + 63) / 64;
+    float q[N];
+    m = -INFINITY; l = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+        const uint32_t d = lane + 64 * c;
+        q[c] = d < a.dim ? element_value<DT>(static_cast<const B*>(a.q)[q_at + d]) : 0.0f;
+        sums[c] = 0.0f;
+    }
+    const uint32_t* row = a.plan.table + (size_t)sequence * a.plan.table_ld;
+    for (uint32_t p = max(begin * 32, lo); p < min(end * 32, hi); p++) {
+        const uint32_t b = p >> a.plan.shift, pg = b < a.plan.table_ld ? row[b] : 0xFFFFFFFFu;
+        if (pg >= a.plan.pages) continue;
+        const size_t at = (((((size_t)pg * a.kv_heads + g) << a.plan.shift) + (p & ((1u << a.plan.shift) - 1))) * D);
+        float s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < N; c++) if (lane + 64 * c < a.dim) s = __builtin_fmaf(q[c], element_value<DT>(static_cast<const B*>(a.keys)[at + lane + 64 * c]), s);
+        s = lh_group_sum(s, 64) * (a.scale * kLog2e);
+        const float nm = fmaxf(m, s), base = nm == -INFINITY ? 0.0f : nm, f = exp2f(m - base), w = exp2f(s - base);
+        l = l * f + w;
+#pragma unroll
+        for (int c = 0; c < N; c++) {
+            const uint32_t d = lane + 64 * c;
+            if (d < a.dim) sums[c] = __builtin_fmaf(w, element_value<DT>(static_cast<const B*>(a.values)[at + d]), sums[c] * f);
+        }
+        m = nm;
+    }
+}
+
+// A workgroup per tile, kv head and split; its four waves take the split's positions in turn, each a quarter of them side by side,
+// straight from global memory; their results meet in LDS.
+//   S^T = K Q^T    a lane has packed row lane & 15 and positions 4 (lane / 16) .. + 3 of both halves of a step
+//   O^T = V^T P^T  the weights are operands where they are; of V a lane loads D / 16 neighbouring columns of its eight positions, and
+//                  pairs of positions are put together in registers, a column per product: no LDS on the way
+// Weights of 16 bits are two terms, what the first leaves being the second.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
+    typedef element_t<DT> B;
+    constexpr bool WIDE = DT == kF32;
+    constexpr int DL = D / 16, kRow = D + 4, KC = WIDE ? D / 16 : D / 32;
+    extern __shared__ __align__(16) float slab[];             // [4 waves][16][kRow]
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gr = lane >> 4, lr = lane & 15;
+    const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = blockIdx.x / a.kv_heads / a.splits;
+    const Tile tile = tile_of<16>(a, t, lane);
+    if (tile.sequence < 0) return;
+    const uint32_t R = a.heads / a.kv_heads, packed = tile.row0 + lr, row = packed / R, head = g * R + packed - row * R;
+    const bool on = lr < tile.count;
+    const uint32_t last_row = (tile.row0 + tile.count - 1) / R, first_row = tile.row0 / R;
+    const Seen mine = seen_by(a, tile, min(row, last_row)), first_seen = seen_by(a, tile, first_row), last_seen = seen_by(a, tile, last_row);
+    const Part part = part_of(a, first_seen.lo, last_seen.hi, z);
+    if (z >= part.used) return;
+    const uint32_t per = (part.end - part.begin + 3) / 4, begin = min(part.begin + wave * per, part.end), end = min(begin + per, part.end);
+    const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
+
+    u32x4 qf[KC];
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+        constexpr uint32_t n = WIDE ? 4 : 8;
+        const uint32_t d = c * 4 * n + gr * n;
+        u32x4 x = {0, 0, 0, 0};
+        if (on && a.q_wide) {
+            if (d < a.dim) x = *reinterpret_cast<const u32x4*>(static_cast<const B*>(a.q) + q_at + d);
+        } else if (on) {
+            B e[n];
+#pragma unroll
+            for (uint32_t i = 0; i < n; i++) e[i] = d + i < a.dim ? static_cast<const B*>(a.q)[q_at + d + i] : (B)0;
+            x = *reinterpret_cast<u32x4*>(e);
+        }
+        qf[c] = x;
+    }
+    const float scale2 = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f;
+    lh_f32x4 o[DL];
+#pragma unroll
+    for (int i = 0; i < DL; i++) o[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
+
+    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, 0, 0};
+    if (begin < end) pages.load(a.plan, (begin * 32) >> a.plan.shift, lane);
+    const uint32_t in_page = (1u << a.plan.shift) - 1;
+    for (uint32_t b = begin; b < end; b++) {
+        uint64_t base[2];                                     // of the page's rows for this kv head, from the half's first slot on
+        bool there[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t p = b * 32 + 16 * h, pg = p < last_seen.hi ? pages.of(a.plan, p >> a.plan.shift, lane) : 0xFFFFFFFFu;
+            there[h] = pg < a.plan.pages;
+            base[h] = (((((uint64_t)(there[h] ? pg : 0u) * a.kv_heads + g) << a.plan.shift) + (p & in_page))) * D;
+        }
+        lh_f32x4 s[2];
+        uint32_t v[2][4][WIDE ? DL : DL / 2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const B* K = static_cast<const B*>(a.keys) + base[h] + lr * D + gr * (WIDE ? 4 : 8);
+            u32x4 kf[KC];
+#pragma unroll
+            for (int c = 0; c < KC; c++) kf[c] = *reinterpret_cast<const u32x4*>(K + c * (WIDE ? 16 : 32));
+            const B* V = static_cast<const B*>(a.values) + base[h] + gr * 4 * D + lr * DL;
+#pragma unroll
+            for (int j = 0; j < 4; j++) load_words(V + j * D, v[h][j]);
+            s[h] = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                if constexpr (WIDE) {
+                    const lh_f32x4 x = __builtin_bit_cast(lh_f32x4, kf[c]), y = __builtin_bit_cast(lh_f32x4, qf[c]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], s[h], 0, 0, 0);
+                } else {
+                    s[h] = product<DT>(kf[c], qf[c], s[h]);
+                }
+            }
+        }
+        float p[8], mx = -INFINITY;
+        const bool whole = b * 32 >= last_seen.lo && b * 32 + 32 <= first_seen.hi && there[0] && there[1];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = s[i >> 2][i & 3] * scale2;
+            if (!whole) {
+                const uint32_t at = b * 32 + (i >> 2) * 16 + gr * 4 + (i & 3);
+                if (at < mine.lo || at >= mine.hi || !there[i >> 2]) p[i] = -INFINITY;
+                if (at >= last_seen.hi || at < first_seen.lo || !there[i >> 2]) {      // seen by none: may be anything
+#pragma unroll
+                    for (int e = 0; e < (WIDE ? DL : DL / 2); e++) v[i >> 2][i & 3][e] = 0;
+                }
+            }
+            mx = fmaxf(mx, p[i]);
+        }
+        const float nm = fmaxf(m, lh_column_max(mx)), base_m = nm == -INFINITY ? 0.0f : nm, alpha = __builtin_amdgcn_exp2f(m - base_m);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(p[i] - base_m); sum += p[i]; }
+        l = l * alpha + sum;                                  // this lane's positions; the four lanes of a row are added at the end
+        m = nm;
+#pragma unroll
+        for (int i = 0; i < DL; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[i][j] *= alpha;
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < DL; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, v[j >> 2][j & 3][i]), p[j], o[i], 0, 0, 0);
+        } else {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                hi[i] = pack2<DT>(p[2 * i], p[2 * i + 1]);
+                lo[i] = pack2<DT>(p[2 * i] - low<DT>(hi[i]), p[2 * i + 1] - high<DT>(hi[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < DL; i++) {
+                const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+                u32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = __builtin_amdgcn_perm(v[e >> 1][(e & 1) * 2 + 1][i / 2], v[e >> 1][(e & 1) * 2][i / 2], sel);
+                o[i] = product<DT>(x, hi, o[i]);
+                o[i] = product<DT>(x, lo, o[i]);
+            }
+        }
+    }
+    // The wave's results: row lr, columns (4 gr + j) DL + i.
+    float* own = slab + wave * 16 * kRow;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < DL; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) odd = odd || o[i][j] != o[i][j];
+    l = lh_column_sum(l);
+    if (__any(on && odd)) {
+        for (uint32_t r = 0; r < tile.count; r++) {
+            const uint32_t pk = tile.row0 + r, rw = pk / R;
+            const Seen sn = seen_by(a, tile, rw);
+            float sm, sl, sums[(D + 63) / 64];
+            slow_row<DT, D>(a, tile.sequence, (uint64_t)(tile.first + rw) * a.q_ld + (uint64_t)(g * R + pk - rw * R) * a.dim, g, sn.lo, sn.hi, begin, end, lane, sm, sl, sums);
+#pragma unroll
+            for (int c = 0; c < (D + 63) / 64; c++) if (lane + 64 * c < D) own[r * kRow + lane + 64 * c] = sums[c];
+            if (lane == 0) { own[r * kRow + D] = sm; own[r * kRow + D + 1] = sl; }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float* to = own + lr * kRow + (4 * gr + j) * DL;
+            if constexpr (DL % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < DL; i += 4) *reinterpret_cast<lh_f32x4*>(to + i) = (lh_f32x4){o[i][j], o[i + 1][j], o[i + 2][j], o[i + 3][j]};
+            } else {
+#pragma unroll
+                for (int i = 0; i < DL; i++) to[i] = o[i][j];
+            }
+        }
+        if (gr == 0) { own[lr * kRow + D] = m; own[lr * kRow + D + 1] = l; }
+    }
+    __syncthreads();
+    const uint32_t r = tid >> 4, c0 = (tid & 15) * 4;
+    if (r >= tile.count) return;
+    float top = -INFINITY, total = 0.0f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++) top = fmaxf(top, slab[(w * 16 + r) * kRow + D]);
+    const uint32_t pk = tile.row0 + r, rw = pk / R, hd = g * R + pk - rw * R;
+    const bool alone = part.used == 1;
+    const float sink = alone && a.sink ? a.sink[hd] * kLog2e : -INFINITY, ref = fmaxf(top, sink), zero = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        f[w] = __builtin_amdgcn_exp2f(slab[(w * 16 + r) * kRow + D] - zero);
+        total += f[w] * slab[(w * 16 + r) * kRow + D + 1];
+    }
+    const float all = total + __builtin_amdgcn_exp2f(sink - zero), inv = alone ? (total == 0.0f ? 0.0f : 1.0f / all) : 1.0f;
+    float* rec = alone ? nullptr : a.partial + (((size_t)(t * a.kv_heads + g) * a.splits + z) * 16 + r) * kRow;
+    if (rec && c0 == 0) { rec[D] = zero; rec[D + 1] = total; }
+    B* out = static_cast<B*>(a.out) + (uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim;
+    for (uint32_t c = c0; c < D; c += 64) {
+        lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const lh_f32x4 y = *reinterpret_cast<const lh_f32x4*>(slab + (w * 16 + r) * kRow + c);
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] += f[w] == 0.0f ? 0.0f : f[w] * y[j];
+        }
+        if (rec) { *reinterpret_cast<lh_f32x4*>(rec + c) = x; continue; }
+#pragma unroll
+        for (int j = 0; j < 4; j++) if (c + j < a.dim) out[c + j] = element_bits<DT>(x[j] * inv);
+    }
+}
+
+// A workgroup per packed row of a tile that several splits have a part of: D / 4 lanes a split, four columns each; groups of lanes take the splits in
+// turn and are added through LDS.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
+    typedef element_t<DT> B;
+    constexpr uint32_t kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS;
+    __shared__ lh_f32x4 sums[256];
+    __shared__ float totals[GROUPS];
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t r = blockIdx.x % 16, g = blockIdx.x / 16 % a.kv_heads, t = blockIdx.x / 16 / a.kv_heads;
+    const Tile tile = tile_of<16>(a, t, lane);
+    if (tile.sequence < 0 || r >= tile.count) return;
+    const uint32_t R = a.heads / a.kv_heads, pk = tile.row0 + r, rw = pk / R, hd = g * R + pk - rw * R;
+    const Part part = part_of(a, seen_by(a, tile, tile.row0 / R).lo, seen_by(a, tile, (tile.row0 + tile.count - 1) / R).hi, 0);
+    if (part.used == 1) return;
+    const float* rec = a.partial + ((size_t)(t * a.kv_heads + g) * a.splits * 16 + r) * kRow;
+    const size_t stride = 16 * kRow;
+    float top = -INFINITY;
+    for (uint32_t s = lane; s < part.used; s += 64) if (rec[s * stride + D + 1] != 0.0f) top = fmaxf(top, rec[s * stride + D]);
+    top = lh_group_max(top, 64);
+    const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY, ref = fmaxf(top, sink), zero = ref == -INFINITY ? 0.0f : ref;
+    const uint32_t grp = tid / QUADS, c = tid % QUADS * 4;
+    lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
+    float total = 0.0f;
+    if (grp < GROUPS) {
+#pragma unroll 4
+        for (uint32_t s = grp; s < part.used; s += GROUPS) {
+            const float* p = rec + s * stride;
+            const float l = p[D + 1], f = __builtin_amdgcn_exp2f(p[D] - zero);
+            const lh_f32x4 y = *reinterpret_cast<const lh_f32x4*>(p + c);
+            if (l != 0.0f) {
+                total += f * l;
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[j] += f == 0.0f ? 0.0f : f * y[j];
+            }
+        }
+        if (c == 0) totals[grp] = total;
+    }
+    sums[tid] = x;
+    __syncthreads();
+    if (tid >= QUADS) return;
+    total = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < GROUPS; i++) total += totals[i];
+#pragma unroll
+    for (uint32_t i = 1; i < GROUPS; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] += sums[i * QUADS + tid][j];
+    const float inv = total == 0.0f ? 0.0f : 1.0f / (total + __builtin_amdgcn_exp2f(sink - zero));
+    B* out = static_cast<B*>(a.out) + (uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim;
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (c + j < a.dim) out[c + j] = element_bits<DT>(x[j] * inv);
+}
+
+// How a launch is cut: tiles of all sequences at most, and parts of a tile's positions.
+struct Cut { uint64_t tiles; uint32_t splits, chunk; };
+Cut cut(uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t window) {
+    const uint32_t R = heads / kv_heads;
+    Cut c;
+    c.tiles = std::min<uint64_t>((uint64_t)rows * R / 16 + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + 15) / 16));
+    uint64_t steps = ((uint64_t)max_length + 31) / 32;
+    if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + 16 + 62) / 32);
+    // as many parts as fill the chip, or more where they would be longer than 32 steps; none shorter than 8.  (More steps never make
+    // fewer parts: a workspace is enough for every window.)
+    const uint64_t units = c.tiles * kv_heads, most = (steps + 7) / 8, fewest = (steps + 31) / 32;
+    c.splits = units >= 4096 ? 1u : (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(2048 / units, fewest), most), 1), 512);
+    c.chunk = (uint32_t)std::max<uint64_t>((steps + c.splits - 1) / c.splits, 1);
+    return c;
+}
+
+template <int DT, int D>
+int launch_rows(lh_context* ctx, const PagedArgs& a, const char* op, uint32_t& launches) {
+    const size_t lds = (size_t)4 * 16 * (D + 4) * 4;
+    int r = lh_raise_dynamic_lds(ctx, (const void*)paged_rows_kernel<DT, D>, lds, op);
+    if (r != LH_OK) return r;
+    hipLaunchKernelGGL((paged_rows_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
+    launches = 1;
+    if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
+    hipLaunchKernelGGL((paged_merge_kernel<DT, D>), dim3(a.tiles * a.kv_heads * 16), dim3(256), 0, ctx->stream, a);
+    launches = 2;
+    return lh_check_launch(op);
+}
+template <int DT>
+int launch_rows(lh_context* ctx, const PagedArgs& a, const char* op, uint32_t& launches) {
+    switch (lh_paged_padded_dim(a.dim)) {
+        case 32: return launch_rows<DT, 32>(ctx, a, op, launches);
+        case 64: return launch_rows<DT, 64>(ctx, a, op, launches);
+        case 128: return launch_rows<DT, 128>(ctx, a, op, launches);
+        case 192: return launch_rows<DT, 192>(ctx, a, op, launches);
+        default: return launch_rows<DT, 256>(ctx, a, op, launches);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t lh_paged_attention_workspace_bytes(uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
+    if (kv_heads == 0 || heads == 0 || heads % kv_heads || dim == 0 || dim > 256 || rows == 0 || sequences == 0 || max_rows == 0) return 0;
+    const Cut c = cut(rows, sequences, max_rows, max_length, heads, kv_heads, 0);
+    return c.splits == 1 ? 0 : (size_t)c.tiles * kv_heads * c.splits * 16 * (lh_paged_padded_dim(dim) + 4) * 4;
+}
+
+int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer* keys, const lh_buffer* values, lh_buffer* output, int dtype, const lh_buffer* table,
+                            const lh_buffer* starts, const lh_buffer* lengths, uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads,
+                            uint32_t kv_heads, uint32_t dim, uint32_t pages, uint32_t page, uint32_t table_ld, uint32_t q_ld, uint32_t output_ld, float scale, uint32_t window,
+                            const lh_buffer* sink, lh_buffer* workspace) {
+    const char* op = "paged_attention";
+    LH_REQUIRE(batch, "%s: batch is null", op);
+    int r = paged_check(op, keys, values, table, starts, lengths, dtype, sequences, kv_heads, dim, pages, page, table_ld);
+    if (r != LH_OK) return r;
+    LH_REQUIRE(heads > 0 && heads <= 65536 && heads % kv_heads == 0, "%s: heads %u is not a multiple of kv_heads %u", op, heads, kv_heads);
+    LH_REQUIRE(std::isfinite(scale), "%s: scale %g", op, (double)scale);
+    if (rows == 0) return LH_OK;
+    LH_REQUIRE(max_rows > 0 && max_rows <= rows, "%s: %u rows, at most %u of a sequence", op, rows, max_rows);
+    LH_REQUIRE((uint64_t)rows * heads < 0x7FFFFFFFull, "%s: %u rows of %u heads", op, rows, heads);
+    const size_t size = lh_dtype_size((lh_dtype)dtype);
+    const uint64_t width = (uint64_t)heads * dim;
+    if ((r = paged_need_rows(op, q, "q", rows, width, q_ld, size)) != LH_OK) return r;
+    if ((r = paged_need_rows(op, output, "output", rows, width, output_ld, size)) != LH_OK) return r;
+    LH_REQUIRE(!paged_rows_meet(q, width, q_ld, output, width, output_ld, rows, size), "%s: q and output overlap", op);
+    PagedArgs a{};
+    if (sink) {
+        LH_NEED(sink, (size_t)heads * 4, op, "sink");
+        LH_REQUIRE(((uintptr_t)sink->ptr & 3) == 0, "%s: sink has to begin at 4 bytes", op);
+        a.sink = (const float*)sink->ptr;
+    }
+    const Cut c = cut(rows, sequences, max_rows, max_length, heads, kv_heads, window);
+    if (c.splits > 1) {
+        const size_t bytes = (size_t)c.tiles * kv_heads * c.splits * 16 * (lh_paged_padded_dim(dim) + 4) * 4;
+        LH_NEED(workspace, bytes, op, "workspace");
+        LH_REQUIRE(((uintptr_t)workspace->ptr & 15) == 0, "%s: workspace has to begin at 16 bytes", op);
+        a.partial = (float*)workspace->ptr;
+    }
+    LH_REQUIRE(c.tiles * kv_heads * std::max(c.splits, 16u) < 0x7FFFFFFFull, "%s: %u rows of %u heads", op, rows, heads);
+    a.q = q->ptr; a.keys = keys->ptr; a.values = values->ptr; a.out = output->ptr;
+    a.plan = PagedPlan{(const uint32_t*)table->ptr, (const uint32_t*)starts->ptr, (const uint32_t*)lengths->ptr, rows, sequences, table_ld, pages, (uint32_t)__builtin_ctz(page)};
+    a.q_ld = q_ld; a.out_ld = output_ld;
+    a.max_rows = max_rows; a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.window = window;
+    a.capacity = (uint32_t)std::min<uint64_t>((uint64_t)table_ld * page, max_length);
+    a.tiles = (uint32_t)c.tiles; a.splits = c.splits; a.chunk = c.chunk;
+    a.q_wide = (((uintptr_t)a.q | (uint64_t)q_ld * size | (uint64_t)dim * size) & 15) == 0;
+    a.out_wide = (((uintptr_t)a.out | (uint64_t)output_ld * size | (uint64_t)dim * size) & 15) == 0;
+    a.scale = scale;
+    uint32_t launches = 0;
+    if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, op, launches);
+    else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, op, launches);
+    else r = launch_rows<kBf16>(batch->ctx, a, op, launches);
+    batch->dispatch_count += launches;
+    return r;
+}
+
+}  // extern "C"

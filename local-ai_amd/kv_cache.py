@@ -3,10 +3,12 @@ in device memory with ring addressing for sliding-window layers."""
 from __future__ import annotations
 
 import ctypes as C
+from dataclasses import dataclass
+from typing import Optional, Sequence
 
 import numpy as np
 
-from . import F32, Buffer, InvalidArgument, Kernels, lib
+from . import BF16, F32, ROTARY_HALVES, Buffer, InvalidArgument, Kernels, lib
 
 TQ_SEED = 0x7459C0DE       # quant_cache.rs:30
 DEFAULT_KV_BITS = 2        # quant_cache.rs:37
@@ -306,6 +308,120 @@ class BlockKvCache:
         """Cleared, not only forgotten: the entries of a block past the last position enter products with weight zero."""
         self.keys.fill_zero()
         self.values.fill_zero()
+
+
+class PageTables:
+    """Which pages of a pool hold which positions of its sequences (host side).  Every layer's ``PagedKvCache`` of a pool goes by the same
+    tables.  Sequences may share whole pages at their beginning: a page goes back when the last of them lets go of it."""
+    NO_PAGE = 0xFFFFFFFF            # the kernels neither write nor see it
+
+    def __init__(self, pages: int, page: int, sequences: int, max_positions: int):
+        if page < 16 or page > 1024 or page & (page - 1):
+            raise InvalidArgument(f"pages of {page} positions, a power of two from 16 to 1024 is wanted")
+        self.page, self.free = page, list(range(pages - 1, -1, -1))
+        self.holders = np.zeros(pages, np.int64)
+        self.table = np.full((sequences, max(-(-max_positions // page), 1)), self.NO_PAGE, np.uint32)
+        self.held = [0] * sequences                 # pages of a sequence
+
+    def reserve(self, sequence: int, positions: int) -> None:
+        """Pages for the sequence's first `positions` positions; all of what lacks or, where the pool has too few, nothing."""
+        need = -(-positions // self.page)
+        if need > self.table.shape[1]:
+            raise InvalidArgument(f"{positions} positions in a table of {self.table.shape[1]} pages of {self.page}")
+        lack = need - self.held[sequence]
+        if lack > len(self.free):
+            raise InvalidArgument(f"{lack} pages wanted, {len(self.free)} free")
+        for b in range(self.held[sequence], need):
+            self.table[sequence, b] = p = self.free.pop()
+            self.holders[p] = 1
+        self.held[sequence] = max(self.held[sequence], need)
+
+    def share(self, source: int, target: int, positions: int) -> int:
+        """Gives an empty sequence the whole pages of the source's first `positions` positions; returns how many positions those hold.  What
+        stands there must be written already: neither sequence may append to them."""
+        if self.held[target]:
+            raise InvalidArgument(f"sequence {target} has pages")
+        n = min(positions // self.page, self.held[source])
+        self.table[target, :n] = self.table[source, :n]
+        self.holders[self.table[source, :n]] += 1
+        self.held[target] = n
+        return n * self.page
+
+    def release(self, sequence: int) -> None:
+        for p in self.table[sequence, :self.held[sequence]]:
+            self.holders[p] -= 1
+            if self.holders[p] == 0:
+                self.free.append(int(p))
+        self.table[sequence] = self.NO_PAGE
+        self.held[sequence] = 0
+
+
+class PagedStep:
+    """A step over sequences of a pool, as the kernels read it: whose the rows are, and where they stand.  Made once for up to `max_rows`
+    rows of a sequence and `max_length` positions; ``write`` puts a step in, ahead of the launches (or a recorded batch) that it is for."""
+
+    def __init__(self, ctx, tables: PageTables, rows: int, max_rows: int, max_length: int):
+        self.tables, self.sequences, self.table_ld = tables, *tables.table.shape
+        self.rows, self.max_rows, self.max_length = rows, max_rows, max_length
+        self.table = Buffer.empty(ctx, tables.table.nbytes)
+        self.starts = Buffer.empty(ctx, 4 * (self.sequences + 1))
+        self.lengths = Buffer.empty(ctx, 4 * self.sequences)
+
+    def write(self, batch, counts: Sequence[int], lengths: Sequence[int]) -> None:
+        """Sequence s brings counts[s] rows (0: it takes no part) and has lengths[s] positions with them."""
+        if len(counts) != self.sequences or len(lengths) != self.sequences:
+            raise InvalidArgument(f"{len(counts)} and {len(lengths)} sequences of {self.sequences}")
+        for n, length, held in zip(counts, lengths, self.tables.held):
+            if n < 0 or n > min(self.max_rows, length):
+                raise InvalidArgument(f"{n} rows of a sequence of {length} positions, at most {self.max_rows} in a step")
+            if n and (length > self.max_length or length > held * self.tables.page):
+                raise InvalidArgument(f"{length} positions in {held} pages of {self.tables.page}, at most {self.max_length} in a step")
+        if sum(counts) > self.rows:
+            raise InvalidArgument(f"{sum(counts)} rows, the step was made for {self.rows}")
+        batch.write(self.table, self.tables.table)
+        batch.write(self.starts, np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32))
+        batch.write(self.lengths, np.asarray(lengths, np.uint32))
+
+
+@dataclass
+class Rotary:
+    """How a layer turns queries and keys by their positions (``Kernels.rotary_frequencies`` makes the frequencies)."""
+    frequencies: Buffer
+    rot: int
+    first: int = 0
+    pairing: int = ROTARY_HALVES
+    amplitude: float = 1.0
+
+
+class PagedKvCache:
+    """Keys and values of one softmax-attention layer for all sequences of a pool, in pages [page][kv head][slot][padded dim].  Nothing has to
+    be cleared: what no sequence has written is not seen."""
+
+    def __init__(self, ctx, kernels: Kernels, kv_heads: int, dim: int, pages: int, page: int, dtype: int = BF16):
+        self.kv_heads, self.dim, self.pages, self.page, self.dtype = kv_heads, dim, pages, page, dtype
+        nbytes = pages * kv_heads * page * kernels.paged_padded_dim(dim) * (4 if dtype == F32 else 2)
+        self.keys, self.values = Buffer.empty(ctx, nbytes), Buffer.empty(ctx, nbytes)
+
+    def append_into(self, batch, kernels: Kernels, step: PagedStep, k: Buffer, v: Buffer, k_ld: int = 0, v_ld: int = 0,
+                    rotary: Optional[Rotary] = None, q: Optional[Buffer] = None, q_output: Optional[Buffer] = None, heads: int = 0, q_ld: int = 0,
+                    q_output_ld: int = 0) -> None:
+        """The step's keys, turned, and values to their pages; its queries turned into `q_output` (may be `q`).  Rows without a distance lie
+        one behind the other."""
+        n, h = self.kv_heads * self.dim, heads * self.dim
+        turn = (rotary.frequencies, rotary.amplitude, rotary.rot, rotary.first, rotary.pairing) if rotary else ()
+        kernels.paged_append_into(batch, k, v, self.dtype, self.keys, self.values, step.table, step.starts, step.lengths, step.rows, step.sequences,
+                                  self.kv_heads, self.dim, self.pages, self.page, step.table_ld, k_ld or n, v_ld or n, *turn, q=q,
+                                  q_output=q_output, heads=heads, q_ld=q_ld or h, q_output_ld=q_output_ld or h)
+
+    def workspace_bytes(self, kernels: Kernels, step: PagedStep, heads: int) -> int:
+        return kernels.paged_attention_workspace_bytes(step.rows, step.sequences, step.max_rows, step.max_length, heads, self.kv_heads, self.dim)
+
+    def attention_into(self, batch, kernels: Kernels, step: PagedStep, q: Buffer, output: Buffer, heads: int, scale: float,
+                       workspace: Optional[Buffer] = None, window: int = 0, sink: Optional[Buffer] = None, q_ld: int = 0, output_ld: int = 0) -> None:
+        h = heads * self.dim
+        kernels.paged_attention_into(batch, q, self.keys, self.values, output, self.dtype, step.table, step.starts, step.lengths, step.rows,
+                                     step.sequences, step.max_rows, step.max_length, heads, self.kv_heads, self.dim, self.pages, self.page,
+                                     step.table_ld, q_ld or h, output_ld or h, scale, window, sink, workspace)
 
 
 class RecurrentState:

@@ -1,7 +1,7 @@
 // The kernel-dispatch layer: `Kernels`, one method per operation of liblocal_hip.so, with the names and the argument
 // order that local-engine calls on local-metal (local-metal/src/kernels.rs).  GENERATED by gen_safe.py from
 // include/local_hip.h: do not edit.  Operations with host pointers and the helpers of the codec are wrapped by hand in lib.rs: lh_matvec_quant_norm_chain_gelu_into, lh_turboquant_levels, lh_turboquant_signs, lh_turboquant_code_bytes, lh_swa_ring_capacity, lh_flash_attention_tq_rotated_lazy_into, lh_token_attention_tq_into, lh_flash_split_count.
-// Other host-side helpers are reached through `ffi`: lh_qk_norm_rope_available, lh_smallm_max_m, lh_batchm_max_m, lh_multivec_max_m, lh_batchm_enabled, lh_mma_enabled, lh_smallm_enabled, lh_kv_bits_from_env, lh_gated_vector_fits, lh_attention_padded_dim, lh_attention_padded_vdim, lh_latent_padded_rank, lh_latent_row, lh_linear_attention_padded_dim, lh_linear_attention_workspace_bytes, lh_selective_steps_bytes, lh_moe_plan_words.
+// Other host-side helpers are reached through `ffi`: lh_qk_norm_rope_available, lh_smallm_max_m, lh_batchm_max_m, lh_multivec_max_m, lh_batchm_enabled, lh_mma_enabled, lh_smallm_enabled, lh_kv_bits_from_env, lh_gated_vector_fits, lh_attention_padded_dim, lh_attention_padded_vdim, lh_latent_padded_rank, lh_latent_row, lh_linear_attention_padded_dim, lh_linear_attention_workspace_bytes, lh_selective_steps_bytes, lh_moe_plan_words, lh_rotary_frequencies, lh_paged_padded_dim, lh_paged_attention_workspace_bytes.
 use core::ffi::c_int;
 
 use crate::batch::CommandBatch;
@@ -770,6 +770,27 @@ impl Kernels {
     pub fn moe_vector_down_into(&self, batch: &mut CommandBatch, hidden: &Buffer, logits: &Buffer, down: &Buffer, residual: &Buffer, experts: u32, top: u32, width: u32, ff: u32) -> Result<()> {
         // SAFETY: every pointer comes from a live handle of this crate; the library validates sizes and shapes.
         check(unsafe { ffi::lh_moe_vector_down_into(batch.as_ptr(), hidden.as_ptr(), logits.as_ptr(), down.as_ptr(), residual.as_ptr(), experts, top, width, ff) })
+    }
+
+    /// `lh_rotary_rows_into` (include/local_hip.h).
+    #[allow(clippy::too_many_arguments)]
+    pub fn rotary_rows_into(&self, batch: &mut CommandBatch, input: &Buffer, output: &Buffer, dtype: c_int, positions: &Buffer, frequencies: &Buffer, amplitude: f32, rows: u32, heads: u32, dim: u32, rot: u32, first: u32, pairing: u32, input_ld: u32, output_ld: u32) -> Result<()> {
+        // SAFETY: every pointer comes from a live handle of this crate; the library validates sizes and shapes.
+        check(unsafe { ffi::lh_rotary_rows_into(batch.as_ptr(), input.as_ptr(), output.as_ptr(), dtype, positions.as_ptr(), frequencies.as_ptr(), amplitude, rows, heads, dim, rot, first, pairing, input_ld, output_ld) })
+    }
+
+    /// `lh_paged_append_into` (include/local_hip.h).
+    #[allow(clippy::too_many_arguments)]
+    pub fn paged_append_into(&self, batch: &mut CommandBatch, k: &Buffer, v: &Buffer, dtype: c_int, keys: &Buffer, values: &Buffer, table: &Buffer, starts: &Buffer, lengths: &Buffer, rows: u32, sequences: u32, kv_heads: u32, dim: u32, pages: u32, page: u32, table_ld: u32, k_ld: u32, v_ld: u32, frequencies: &Buffer, amplitude: f32, rot: u32, first: u32, pairing: u32, q: &Buffer, q_output: &Buffer, heads: u32, q_ld: u32, q_output_ld: u32) -> Result<()> {
+        // SAFETY: every pointer comes from a live handle of this crate; the library validates sizes and shapes.
+        check(unsafe { ffi::lh_paged_append_into(batch.as_ptr(), k.as_ptr(), v.as_ptr(), dtype, keys.as_ptr(), values.as_ptr(), table.as_ptr(), starts.as_ptr(), lengths.as_ptr(), rows, sequences, kv_heads, dim, pages, page, table_ld, k_ld, v_ld, frequencies.as_ptr(), amplitude, rot, first, pairing, q.as_ptr(), q_output.as_ptr(), heads, q_ld, q_output_ld) })
+    }
+
+    /// `lh_paged_attention_into` (include/local_hip.h).
+    #[allow(clippy::too_many_arguments)]
+    pub fn paged_attention_into(&self, batch: &mut CommandBatch, q: &Buffer, keys: &Buffer, values: &Buffer, output: &Buffer, dtype: c_int, table: &Buffer, starts: &Buffer, lengths: &Buffer, rows: u32, sequences: u32, max_rows: u32, max_length: u32, heads: u32, kv_heads: u32, dim: u32, pages: u32, page: u32, table_ld: u32, q_ld: u32, output_ld: u32, scale: f32, window: u32, sink: &Buffer, workspace: &Buffer) -> Result<()> {
+        // SAFETY: every pointer comes from a live handle of this crate; the library validates sizes and shapes.
+        check(unsafe { ffi::lh_paged_attention_into(batch.as_ptr(), q.as_ptr(), keys.as_ptr(), values.as_ptr(), output.as_ptr(), dtype, table.as_ptr(), starts.as_ptr(), lengths.as_ptr(), rows, sequences, max_rows, max_length, heads, kv_heads, dim, pages, page, table_ld, q_ld, output_ld, scale, window, sink.as_ptr(), workspace.as_ptr()) })
     }
 
     /// `lh_advance_position_into` (include/local_hip.h).

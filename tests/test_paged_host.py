@@ -1,0 +1,218 @@
+"""Host side of rotary positions and paged caches: frequencies, page tables, workspaces and every refusal.  No GPU work: the entry points
+refuse before they touch a device, so the buffers here are handles over no memory."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from paged_models import padded
+
+
+# ---- frequencies ------------------------------------------------------------------------------------------------------------
+def by_parts(rot, base, factor, original, fast, slow):
+    def index(turns):
+        return rot * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+    lo, hi = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rot - 1)
+    i = np.arange(rot // 2)
+    f = base ** (-2.0 * i / rot)
+    ramp = np.clip((i - lo) / (max(hi - lo, 0.001)), 0, 1)
+    return f * (1 - ramp) + f / factor * ramp
+
+
+@pytest.mark.parametrize("rot,base", [(2, 1e4), (50, 1e4), (128, 1e6), (256, 5e5)])
+def test_frequencies_follow_their_formulas(pkg, rot, base):
+    K = pkg.Kernels
+    f, a = K.rotary_frequencies(rot, base)
+    want = base ** (-2.0 * np.arange(rot // 2) / rot)
+    assert a == 1.0 and f.dtype == np.float32 and np.allclose(f, want, rtol=2.0 ** -23, atol=0)
+    f, a = K.rotary_frequencies(rot, base, pkg.ROTARY_LINEAR, 8.0)
+    assert a == 1.0 and np.allclose(f, want / 8, rtol=2.0 ** -23, atol=0)
+    f, a = K.rotary_frequencies(rot, base, pkg.ROTARY_BY_PARTS, 4.0, 4096.0, 32.0, 1.0)
+    assert a == np.float32(0.1 * math.log(4.0) + 1.0) and np.allclose(f, by_parts(rot, base, 4.0, 4096.0, 32.0, 1.0), rtol=2.0 ** -22, atol=0)
+    assert np.isclose(f[0], 1.0) and np.all(f <= want.astype(np.float32) * (1 + 2.0 ** -22)) and np.all(f >= want / 4 * (1 - 2.0 ** -22))
+
+
+@pytest.mark.parametrize("args", [(0, 1e4), (3, 1e4), (4098, 1e4), (64, 1.0), (64, math.nan), (64, math.inf), (64, 1e4, 3), (64, 1e4, 1, 0.5), (64, 1e4, 1, math.nan),
+                                  (64, 1e4, 2, 4.0, 0.0), (64, 1e4, 2, 4.0, 4096.0, 1.0, 1.0), (64, 1e4, 2, 4.0, 4096.0, 32.0, 0.0),
+                                  (64, 1e4, 2, 4.0, math.inf)])
+def test_frequencies_that_are_refused(pkg, args):
+    with pytest.raises(pkg.InvalidArgument):
+        pkg.Kernels.rotary_frequencies(*args)
+
+
+# ---- page tables --------------------------------------------------------------------------------------------------------------
+def test_tables_deal_out_and_take_back_pages(pkg):
+    from local_ai_amd.kv_cache import PageTables
+    t = PageTables(10, 16, 3, 100)
+    assert t.table.shape == (3, 7) and np.all(t.table == t.NO_PAGE)
+    t.reserve(0, 1)
+    t.reserve(0, 16)
+    assert t.held[0] == 1
+    t.reserve(0, 17)
+    t.reserve(1, 100)
+    assert t.held == [2, 7, 0] and len(t.free) == 1
+    used = np.concatenate([t.table[0, :2], t.table[1]])
+    assert len(set(used.tolist())) == 9 and used.max() < 10
+    with pytest.raises(pkg.InvalidArgument):
+        t.reserve(2, 17)
+    assert t.held[2] == 0 and len(t.free) == 1          # nothing of it is kept
+    with pytest.raises(pkg.InvalidArgument):
+        t.reserve(0, 113)
+    t.release(1)
+    t.reserve(2, 100)
+    t.reserve(2, 5)                                      # never fewer
+    assert t.held == [2, 0, 7] and np.all(t.table[1] == t.NO_PAGE)
+
+
+def test_shared_pages_go_back_with_their_last_holder(pkg):
+    from local_ai_amd.kv_cache import PageTables
+    t = PageTables(8, 16, 3, 64)
+    t.reserve(0, 40)
+    assert t.share(0, 1, 40) == 32 and t.held[1] == 2 and np.array_equal(t.table[0, :2], t.table[1, :2])
+    t.reserve(1, 40)
+    assert t.table[1, 2] != t.table[0, 2]
+    with pytest.raises(pkg.InvalidArgument):
+        t.share(0, 1, 16)
+    assert t.share(1, 2, 15) == 0
+    first = set(t.table[0, :2].tolist())
+    t.release(0)
+    assert not first & set(t.free) and len(t.free) == 5
+    t.release(1)
+    assert first <= set(t.free) and len(t.free) == 8 and not t.holders.any()
+    for page in (0, 8, 24, 2048):
+        with pytest.raises(pkg.InvalidArgument):
+            PageTables(8, page, 1, 64)
+
+
+def test_steps_that_are_refused(pkg, monkeypatch):
+    from local_ai_amd import kv_cache
+    written = []
+
+    class Fake:
+        @staticmethod
+        def empty(ctx, n):
+            return n
+
+    class Batch:
+        def write(self, dst, src):
+            written.append((dst, np.array(src)))
+    monkeypatch.setattr(kv_cache, "Buffer", Fake)
+    t = kv_cache.PageTables(8, 16, 3, 64)
+    t.reserve(0, 33)
+    t.reserve(2, 16)
+    s = kv_cache.PagedStep(None, t, rows=6, max_rows=4, max_length=40)
+    s.write(Batch(), [4, 0, 2], [33, 0, 16])
+    assert [w[1].tolist() for w in written[1:]] == [[0, 4, 4, 6], [33, 0, 16]] and np.array_equal(written[0][1], t.table)
+    for counts, lengths in (([4, 0], [33, 0]), ([5, 0, 0], [33, 0, 0]), ([1, 1, 0], [33, 1, 0]), ([1, 0, 0], [49, 0, 0]), ([3, 0, 0], [2, 0, 0]),
+                            ([4, 0, 3], [33, 0, 16]), ([-1, 0, 0], [33, 0, 0])):
+        with pytest.raises(pkg.InvalidArgument):
+            s.write(Batch(), counts, lengths)
+    t.reserve(0, 48)
+    with pytest.raises(pkg.InvalidArgument):
+        s.write(Batch(), [1, 0, 0], [41, 0, 0])
+
+
+# ---- workspaces -----------------------------------------------------------------------------------------------------------------
+def test_padded_heads_and_workspaces(pkg):
+    lib = pkg.lib()
+    for d in (1, 31, 32, 33, 64, 65, 100, 128, 129, 192, 193, 256):
+        assert lib.lh_paged_padded_dim(d) == padded(d)
+    f = lib.lh_paged_attention_workspace_bytes
+    assert f(1, 1, 1, 64, 8, 2, 128) == 0                     # too short to be cut
+    assert f(1, 1, 1, 32768, 8, 2, 128) > 0
+    assert f(1, 1, 1, 32768, 8, 3, 128) == 0 and f(0, 1, 1, 99, 8, 2, 128) == 0 and f(1, 1, 1, 32768, 8, 0, 128) == 0
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------------------------
+class BufferHandle(C.Structure):          # lh_buffer of csrc/common.hpp
+    _fields_ = [("ctx", C.c_void_p), ("ptr", C.c_void_p), ("len", C.c_size_t), ("owns", C.c_bool), ("slack", C.c_size_t), ("host", C.c_void_p)]
+
+
+class BatchHandle(C.Structure):
+    _fields_ = [("ctx", C.c_void_p), ("dispatch_count", C.c_uint32)]
+
+
+def buf(at, nbytes):
+    return BufferHandle(None, at, nbytes, False, 0, None)
+
+
+GB = 1 << 30
+
+
+class Call:
+    """Arguments of a call that would be taken, by name and in order; `refused` changes some of them."""
+
+    def __init__(self, pkg, name, **args):
+        self.pkg, self.f, self.args = pkg, getattr(pkg.lib(), name), args
+
+    def status(self, **changed):
+        assert set(changed) <= set(self.args)
+        batch = BatchHandle(None, 0)
+        vals = [None if changed.get("batch", 0) is None else C.byref(batch)] if "batch" in self.args else []
+        for name, v in {**self.args, **changed}.items():
+            if name == "batch":
+                continue
+            vals.append(C.byref(v) if isinstance(v, BufferHandle) else C.c_float(v) if isinstance(v, float) else None if v is None else C.c_uint32(v))
+        rc = self.f(*vals)
+        assert batch.dispatch_count == 0
+        return rc
+
+    def refused(self, **changed):
+        assert self.status(**changed) == self.pkg.InvalidArgument.code, changed
+        assert self.pkg.lib().lh_last_error().decode().startswith("Invalid argument: ")
+
+
+def test_rotary_refusals(pkg):
+    c = Call(pkg, "lh_rotary_rows_into", batch=True, input=buf(GB, 10 * 512 * 2), output=buf(2 * GB, 10 * 512 * 2), dtype=2, positions=buf(3 * GB, 40), frequencies=buf(4 * GB, 256),
+             amplitude=1.0, rows=10, heads=4, dim=128, rot=128, first=0, pairing=1, input_ld=512, output_ld=512)
+    assert c.status(rows=0) == 0 and c.status(heads=0) == 0
+    for changed in (dict(batch=None), dict(dtype=3), dict(dtype=1), dict(rot=127), dict(rot=130), dict(rot=64, first=65), dict(first=2), dict(pairing=2), dict(dim=0), dict(dim=2048),
+                    dict(input=None), dict(output=None), dict(positions=None), dict(frequencies=None), dict(rows=11), dict(heads=5), dict(input_ld=511), dict(output_ld=500),
+                    dict(input_ld=513), dict(positions=buf(3 * GB, 39)), dict(frequencies=buf(4 * GB, 255)), dict(input=buf(GB + 1, 10 * 512 * 2)),
+                    dict(heads=1 << 20), dict(output=buf(GB + 2, 10 * 512 * 2)), dict(output=buf(GB + 1024, 10 * 512 * 2)),
+                    dict(positions=buf(3 * GB + 2, 40)), dict(frequencies=buf(4 * GB + 1, 256)), dict(first=0xFFFFFFFE)):
+        c.refused(**changed)
+    # the same rows at another distance; rows of one distance side by side are taken (checked on the device)
+    c.refused(output=buf(GB, 10 * 600 * 2), output_ld=600)
+
+
+def append_call(pkg, **more):
+    pool = 7 * 2 * 16 * 128 * 2
+    a = dict(batch=True, k=buf(GB, 6 * 1024 * 2), v=buf(2 * GB, 6 * 1024 * 2), dtype=2, keys=buf(3 * GB, pool), values=buf(4 * GB, pool), table=buf(5 * GB, 3 * 4 * 4),
+             starts=buf(6 * GB, 16), lengths=buf(7 * GB, 12), rows=6, sequences=3, kv_heads=2, dim=100, pages=7, page=16, table_ld=4, k_ld=1024, v_ld=1024,
+             frequencies=buf(8 * GB, 200), amplitude=1.0, rot=100, first=0, pairing=0, q=buf(9 * GB, 6 * 800 * 2), q_output=buf(10 * GB, 6 * 800 * 2), heads=8, q_ld=800, q_output_ld=800)
+    return Call(pkg, "lh_paged_append_into", **{**a, **more})
+
+
+def test_append_refusals(pkg):
+    c = append_call(pkg)
+    assert c.status(rows=0) == 0
+    pool = 7 * 2 * 16 * 128 * 2
+    for changed in (dict(batch=None), dict(dtype=4), dict(dtype=1), dict(k=None), dict(v=None), dict(keys=None), dict(values=None), dict(table=None), dict(starts=None),
+                    dict(lengths=None), dict(rows=7), dict(sequences=0), dict(sequences=4), dict(kv_heads=0), dict(kv_heads=3), dict(dim=0), dict(dim=257), dict(dim=129),
+                    dict(pages=0), dict(pages=8), dict(page=8), dict(page=24), dict(page=32), dict(page=2048), dict(table_ld=0), dict(table_ld=5), dict(k_ld=199), dict(v_ld=199),
+                    dict(k_ld=1300), dict(frequencies=None), dict(rot=101), dict(rot=102), dict(first=2), dict(pairing=2), dict(q=None), dict(q_output=None), dict(heads=0),
+                    dict(q=None, q_output=None), dict(heads=9), dict(q_ld=799), dict(q_output_ld=900), dict(keys=buf(3 * GB + 8, pool)), dict(values=buf(3 * GB, pool)),
+                    dict(values=buf(3 * GB + pool - 16, pool)), dict(k=buf(3 * GB + 64, 6 * 1024 * 2)), dict(v=buf(4 * GB - 16, 6 * 1024 * 2)), dict(q=buf(3 * GB, 6 * 800 * 2)),
+                    dict(q_output=buf(4 * GB + pool - 2, 6 * 800 * 2)), dict(q_output=buf(9 * GB + 2, 6 * 800 * 2)), dict(q_output=buf(GB + 398, 6 * 1024 * 2), q_output_ld=1024),
+                    dict(q_output=buf(2 * GB, 6 * 800 * 2)), dict(k=buf(GB + 1, 6 * 1024 * 2)), dict(table=buf(5 * GB + 2, 48)), dict(starts=buf(6 * GB + 1, 16)),
+                    dict(table_ld=1 << 28, page=1024), dict(sequences=1 << 21)):
+        c.refused(**changed)
+    append_call(pkg, q=None, q_output=None, heads=0).refused(q=buf(9 * GB, 6 * 800 * 2))
+
+
+def test_attention_refusals(pkg):
+    pool = 2000 * 2 * 16 * 128 * 2
+    need = pkg.lib().lh_paged_attention_workspace_bytes(6, 3, 4, 16000, 8, 2, 100)
+    assert need > 0
+    c = Call(pkg, "lh_paged_attention_into", batch=True, q=buf(GB, 6 * 800 * 2), keys=buf(3 * GB, pool), values=buf(4 * GB, pool), output=buf(2 * GB, 6 * 800 * 2), dtype=2,
+             table=buf(5 * GB, 3 * 1000 * 4), starts=buf(6 * GB, 16), lengths=buf(7 * GB, 12), rows=6, sequences=3, max_rows=4, max_length=16000, heads=8, kv_heads=2, dim=100,
+             pages=2000, page=16, table_ld=1000, q_ld=800, output_ld=800, scale=0.1, window=0, sink=buf(8 * GB, 32), workspace=buf(9 * GB, need))
+    assert c.status(rows=0) == 0
+    for changed in (dict(batch=None), dict(dtype=7), dict(dtype=1), dict(q=None), dict(keys=None), dict(values=None), dict(output=None), dict(table=None), dict(starts=None),
+                    dict(lengths=None), dict(rows=7), dict(sequences=4), dict(sequences=0), dict(max_rows=0), dict(max_rows=7), dict(heads=0), dict(heads=7), dict(kv_heads=3), dict(kv_heads=0),
+                    dict(dim=0), dict(dim=101), dict(dim=300), dict(pages=2001), dict(page=17), dict(table_ld=1001), dict(q_ld=700), dict(output_ld=799), dict(output_ld=801),
+                    dict(scale=math.nan), dict(scale=math.inf), dict(sink=buf(8 * GB, 31)), dict(sink=buf(8 * GB + 2, 32)), dict(workspace=None), dict(workspace=buf(9 * GB, need - 1)),
+                    dict(workspace=buf(9 * GB + 4, need)), dict(output=buf(GB, 6 * 800 * 2)), dict(output=buf(GB + 6 * 1600 - 2, 6 * 800 * 2)), dict(keys=buf(3 * GB + 2, pool))):
+        c.refused(**changed)
