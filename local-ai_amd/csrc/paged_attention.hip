@@ -3,8 +3,8 @@
 //
 //   out = sum_j softmax_j(scale q . k_j [, sink]) v_j   over the positions j up to the row's own, the last `window` of them where there is one
 //
-// A tile is 16 packed rows (row of the sequence, head of the group) of one kv head; the tiles of all sequences are counted off from
-// `starts` by every wave.  Running maximum and sum in 32 bits, in powers of two.
+// A tile is 16 or 128 packed rows (row of the sequence, head of the group) of one kv head; the tiles of all sequences are counted off
+// from `starts` by every wave.  Running maximum and sum in 32 bits, in powers of two.
 #include "paged.hpp"
 #include <algorithm>
 #include <cmath>
@@ -20,13 +20,14 @@ struct PagedArgs {
     const void *q, *keys, *values;
     void* out;
     const float* sink;         // [heads], may be null
-    float* partial;            // records [tile][kv head][split][16][D + 4]: unnormalised sums, maximum, sum of weights
+    float* partial;            // records [tile][kv head][split][row of the tile][D + 4]: unnormalised sums, maximum, sum of weights
     PagedPlan plan;
     uint64_t q_ld, out_ld;
     uint32_t max_rows, heads, kv_heads, dim, window, capacity;     // capacity: positions from there on are not seen
-    uint32_t tiles, splits, chunk;                                 // chunk: steps of 32 positions that a split takes at least
+    uint32_t tiles, splits, chunk;                                 // chunk: steps that a split takes at least
     uint32_t q_wide, out_wide;                                     // rows, heads and their ends at 16 bytes
-    float scale;
+    float scale2;              // of the products, in powers of two; > 0
+    uint32_t negative, nothing;                                    // the scale is below zero, or zero: in the queries
 };
 
 // A tile of a sequence: its rows row0 .. row0 + count - 1 of the packed ones.
@@ -82,10 +83,11 @@ __device__ __forceinline__ Seen seen_by(const PagedArgs& a, const Tile& t, uint3
     return s;
 }
 
-// The part of a tile's positions that split z takes, in steps of 32; `used` splits have any.
+// The part of a tile's positions that split z takes, in steps of STEP; `used` splits have any.
 struct Part { uint32_t begin, end, used; };
+template <uint32_t STEP>
 __device__ __forceinline__ Part part_of(const PagedArgs& a, uint32_t lo, uint32_t hi, uint32_t z) {
-    const uint32_t b0 = lo / 32, b1 = max((hi + 31) / 32, b0), n = b1 - b0;
+    const uint32_t b0 = lo / STEP, b1 = max((hi + STEP - 1) / STEP, b0), n = b1 - b0;
     const uint32_t used = min(max((n + a.chunk - 1) / a.chunk, 1u), a.splits), per = (n + used - 1) / used;
     return Part{min(b0 + z * per, b1), min(b0 + (z + 1) * per, b1), used};
 }
@@ -134,11 +136,31 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t (&x)[N]) {
     }
 }
 
-// One packed row over steps begin .. end - 1, by one wave and value by value: what takes the place of the matrix instructions where a
+// 16 bytes of a query from column d on, zeros behind its end; the scale's sign goes into it.
+template <int DT>
+__device__ __forceinline__ u32x4 query_words(const PagedArgs& a, uint64_t q_at, uint32_t d, bool on) {
+    typedef element_t<DT> B;
+    constexpr uint32_t n = 16 / sizeof(B);
+    u32x4 x = {0, 0, 0, 0};
+    if (!on || a.nothing) return x;
+    if (a.q_wide) {
+        if (d < a.dim) x = *reinterpret_cast<const u32x4*>(static_cast<const B*>(a.q) + q_at + d);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < n; i++)
+            if (d + i < a.dim) x[i * sizeof(B) / 4] |= (uint32_t)static_cast<const B*>(a.q)[q_at + d + i] << (DT == kF32 ? 0 : 16 * (i & 1));
+    }
+    if (a.negative)
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] ^= DT == kF32 ? 0x80000000u : 0x80008000u;
+    return x;
+}
+
+// One packed row over positions begin .. end - 1, by one wave and value by value: what takes the place of the matrix instructions where a
 // result is not a number.  There a position that a row does not see has the weight 0, and 0 times an infinity or NaN that stands in it
 // is NaN; here it is left out.  Every lane gets the maximum (in powers of two) and the sum; sums[c] is of column lane + 64 c.
 template <int DT, int D>
-__device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint64_t q_at, uint32_t g, uint32_t lo, uint32_t hi, uint32_t begin, uint32_t end, uint32_t lane,
+__device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint64_t q_at, uint32_t g, uint32_t begin, uint32_t end, uint32_t lane,
                                                    float& m, float& l, float (&sums)[(D + 63) / 64]) {
     typedef element_t<DT> B;
     constexpr int N = (D + 63) / 64;
@@ -151,14 +173,14 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint6
         sums[c] = 0.0f;
     }
     const uint32_t* row = a.plan.table + (size_t)sequence * a.plan.table_ld;
-    for (uint32_t p = max(begin * 32, lo); p < min(end * 32, hi); p++) {
+    for (uint32_t p = begin; p < end; p++) {
         const uint32_t b = p >> a.plan.shift, pg = b < a.plan.table_ld ? row[b] : 0xFFFFFFFFu;
         if (pg >= a.plan.pages) continue;
         const size_t at = (((((size_t)pg * a.kv_heads + g) << a.plan.shift) + (p & ((1u << a.plan.shift) - 1))) * D);
         float s = 0.0f;
 #pragma unroll
         for (int c = 0; c < N; c++) if (lane + 64 * c < a.dim) s = __builtin_fmaf(q[c], element_value<DT>(static_cast<const B*>(a.keys)[at + lane + 64 * c]), s);
-        s = lh_group_sum(s, 64) * (a.scale * kLog2e);
+        s = lh_group_sum(s, 64) * (a.nothing ? 0.0f : a.negative ? -a.scale2 : a.scale2);
         const float nm = fmaxf(m, s), base = nm == -INFINITY ? 0.0f : nm, f = exp2f(m - base), w = exp2f(s - base);
         l = l * f + w;
 #pragma unroll
@@ -190,28 +212,15 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
     const bool on = lr < tile.count;
     const uint32_t last_row = (tile.row0 + tile.count - 1) / R, first_row = tile.row0 / R;
     const Seen mine = seen_by(a, tile, min(row, last_row)), first_seen = seen_by(a, tile, first_row), last_seen = seen_by(a, tile, last_row);
-    const Part part = part_of(a, first_seen.lo, last_seen.hi, z);
+    const Part part = part_of<32>(a, first_seen.lo, last_seen.hi, z);
     if (z >= part.used) return;
     const uint32_t per = (part.end - part.begin + 3) / 4, begin = min(part.begin + wave * per, part.end), end = min(begin + per, part.end);
     const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
 
     u32x4 qf[KC];
 #pragma unroll
-    for (int c = 0; c < KC; c++) {
-        constexpr uint32_t n = WIDE ? 4 : 8;
-        const uint32_t d = c * 4 * n + gr * n;
-        u32x4 x = {0, 0, 0, 0};
-        if (on && a.q_wide) {
-            if (d < a.dim) x = *reinterpret_cast<const u32x4*>(static_cast<const B*>(a.q) + q_at + d);
-        } else if (on) {
-            B e[n];
-#pragma unroll
-            for (uint32_t i = 0; i < n; i++) e[i] = d + i < a.dim ? static_cast<const B*>(a.q)[q_at + d + i] : (B)0;
-            x = *reinterpret_cast<u32x4*>(e);
-        }
-        qf[c] = x;
-    }
-    const float scale2 = a.scale * kLog2e;
+    for (int c = 0; c < KC; c++) qf[c] = query_words<DT>(a, q_at, (c * 4 + gr) * (WIDE ? 4 : 8), on);
+    const float scale2 = a.scale2;
     float m = -INFINITY, l = 0.0f;
     lh_f32x4 o[DL];
 #pragma unroll
@@ -313,7 +322,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
             const uint32_t pk = tile.row0 + r, rw = pk / R;
             const Seen sn = seen_by(a, tile, rw);
             float sm, sl, sums[(D + 63) / 64];
-            slow_row<DT, D>(a, tile.sequence, (uint64_t)(tile.first + rw) * a.q_ld + (uint64_t)(g * R + pk - rw * R) * a.dim, g, sn.lo, sn.hi, begin, end, lane, sm, sl, sums);
+            slow_row<DT, D>(a, tile.sequence, (uint64_t)(tile.first + rw) * a.q_ld + (uint64_t)(g * R + pk - rw * R) * a.dim, g, max(begin * 32, sn.lo), min(end * 32, sn.hi), lane, sm, sl, sums);
 #pragma unroll
             for (int c = 0; c < (D + 63) / 64; c++) if (lane + 64 * c < D) own[r * kRow + lane + 64 * c] = sums[c];
             if (lane == 0) { own[r * kRow + D] = sm; own[r * kRow + D + 1] = sl; }
@@ -364,33 +373,265 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
     }
 }
 
-// A workgroup per packed row of a tile that several splits have a part of: D / 4 lanes a split, four columns each; groups of lanes take the splits in
-// turn and are added through LDS.
+typedef float lh_f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+// 16 bytes a lane from base + from straight to LDS, lane by lane from byte `to` on (the same in all lanes).  No registers are written, so
+// nothing can be read too early but LDS itself, behind wait_for_loads and a barrier.  (With the builtin for it the compiler has every
+// transposing read wait for all such loads, the next step's among them.  m0 is the compiler's own and holds nothing over an instruction.)
+__device__ __forceinline__ void load_to_lds(uint32_t to, const void* base, uint32_t from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(from), "s"(base) : "memory");
+}
+// (The builtin tells the compiler, too, that its own loads are there: else it would wait for them, and with them for these, at their first use.)
+__device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); asm volatile("" ::: "memory"); }
+
+template <int DT>
+__device__ __forceinline__ lh_f32x16 product(u32x4 x, u32x4 y, lh_f32x16 c) {
+    if constexpr (DT == kF16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lh_f16x8, x), __builtin_bit_cast(lh_f16x8, y), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lh_bf16x8, x), __builtin_bit_cast(lh_bf16x8, y), c, 0, 0, 0);
+}
+
+// Many rows, 16-bit types: a workgroup per tile of 128 packed rows, kv head and split.  Each of its four waves has 32 rows, all of them
+// share the steps of KT positions, whose keys and values go from memory to LDS without registers, the next step's while this one is used.
+//   S^T = K Q^T    32 x 32 x 16: a lane has packed row lane & 31 and half of the positions, so maximum and sum are its own registers'
+//   O^T = V^T P^T  the weights are operands where they are; V, in LDS as it is in memory, is read by the transposing ds_read_b64_tr_b16
+// In LDS the 16-byte pieces of a row change places by the row's low bits, so that neither read meets itself in a bank: a key's piece c is
+// at c ^ (row & 7), a value's at c ^ 4 (row & 3).
 template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void paged_tiles_kernel(const PagedArgs a) {
+    typedef element_t<DT> B;
+    constexpr uint32_t KT = D <= 128 ? 64 : 32, SUB = KT / 32, KC = D / 16, TD = D / 32, CR = D / 8, PART = KT / 4, LOADS = PART * D / 512, kRow = D + 4;
+    constexpr uint32_t VSWAP = CR % 16 == 0 ? 3 : CR % 8 == 0 ? 1 : 0;
+    extern __shared__ __align__(16) uint16_t stage[];         // [2][keys, values][KT][D]
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, lr = lane & 31;
+    const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = a.tiles - 1 - blockIdx.x / a.kv_heads / a.splits;    // long tiles first
+    const Tile tile = tile_of<128>(a, t, lane);
+    if (tile.sequence < 0) return;
+    const uint32_t R = a.heads / a.kv_heads, last_row = (tile.row0 + tile.count - 1) / R;
+    const Seen first_seen = seen_by(a, tile, tile.row0 / R), last_seen = seen_by(a, tile, last_row);
+    const Part part = part_of<KT>(a, first_seen.lo, last_seen.hi, z);
+    if (z >= part.used) return;
+    // the wave's rows
+    const bool busy = wave * 32 < tile.count;
+    const uint32_t in_tile = min(wave * 32 + lr, tile.count - 1), packed = tile.row0 + in_tile, row = packed / R, head = g * R + packed - row * R;
+    const bool on = wave * 32 + lr < tile.count;
+    const Seen mine = seen_by(a, tile, row), wave_first = seen_by(a, tile, min((tile.row0 + wave * 32) / R, last_row)),
+               wave_last = seen_by(a, tile, (tile.row0 + min(wave * 32 + 31, tile.count - 1)) / R);
+    const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
+    u32x4 qf[KC];
+#pragma unroll
+    for (uint32_t c = 0; c < KC; c++) qf[c] = query_words<DT>(a, q_at, c * 16 + half * 8, on);
+
+    // where a lane's pieces come from, in bytes from the part's first row on
+    uint32_t kfrom[LOADS], vfrom[LOADS];
+#pragma unroll
+    for (uint32_t j = 0; j < LOADS; j++) {
+        const uint32_t id = j * 64 + lane, r = id / CR, c = id % CR, k = CR >= 8 ? (wave * PART + r) & 7 : ((wave * PART + r) >> 1) & 3;
+        kfrom[j] = (r * D + (c ^ k) * 8) * 2;
+        vfrom[j] = (r * D + (c ^ (((wave * PART + r) & VSWAP) << 2)) * 8) * 2;
+    }
+    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, 0, 0};
+    const uint32_t in_page = (1u << a.plan.shift) - 1;
+    if (part.begin < part.end) pages.load(a.plan, (part.begin * KT) >> a.plan.shift, lane);
+    // Requests step b into buffer `at`; returns which quarters of it are there.
+    auto request = [&](uint32_t b, uint32_t at) __attribute__((always_inline)) {
+        uint32_t there = 0, own = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t p = b * KT + i * PART, pg = p < last_seen.hi ? pages.of(a.plan, p >> a.plan.shift, lane) : 0xFFFFFFFFu;
+            if (pg < a.plan.pages) there |= 1u << i;
+            if (i == wave) own = pg < a.plan.pages ? pg : 0u;
+        }
+        const uint64_t base = ((((uint64_t)own * a.kv_heads + g) << a.plan.shift) + ((b * KT + wave * PART) & in_page)) * D;
+        const B *K = static_cast<const B*>(a.keys) + base, *V = static_cast<const B*>(a.values) + base;
+        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)(stage + (at * 2 * KT + wave * PART) * D));
+#pragma unroll
+        for (uint32_t j = 0; j < LOADS; j++) load_to_lds(to + j * 1024, K, kfrom[j]);
+#pragma unroll
+        for (uint32_t j = 0; j < LOADS; j++) load_to_lds(to + KT * D * 2 + j * 1024, V, vfrom[j]);
+        return there;
+    };
+    // where a lane reads operands, in values: of keys row lr, of values row 4 half + (lane & 15) / 4
+    constexpr uint32_t KO = CR >= 8 ? 4 : 2, VO = VSWAP == 3 ? 4 : VSWAP == 1 ? 2 : 1;
+    uint32_t kat[KO], vat[VO];
+#pragma unroll
+    for (uint32_t c = 0; c < KO; c++) kat[c] = lr * D + ((c * 2 + half) ^ (CR >= 8 ? lr & 7 : (lr >> 1) & 3)) * 8;
+#pragma unroll
+    for (uint32_t c = 0; c < VO; c++) {
+        const uint32_t i = lane & 15, r = 4 * half + (i >> 2), piece = c * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+        vat[c] = r * D + (piece ^ ((r & VSWAP) << 2)) * 8 + (i & 1) * 4;
+    }
+
+    const float scale2 = a.scale2;
+    float m = -INFINITY, l = 0.0f;
+    lh_f32x16 o[TD];
+#pragma unroll
+    for (uint32_t d = 0; d < TD; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    uint32_t next_there = part.begin < part.end ? request(part.begin, 0) : 0u;
+    for (uint32_t b = part.begin; b < part.end; b++) {
+        const uint32_t at = (b - part.begin) & 1, there = next_there, p0 = b * KT;
+        wait_for_loads();
+        __syncthreads();                                      // the step is there, and nobody reads the other buffer any more
+        if (b + 1 < part.end) next_there = request(b + 1, at ^ 1);
+        const uint16_t *K = stage + at * 2 * KT * D, *V = K + KT * D;
+        if (p0 + KT > last_seen.hi || p0 < first_seen.lo || there != 15u) {      // positions that no row sees: what stands there may be anything
+            uint16_t* v = stage + (at * 2 + 1) * KT * D;
+            for (uint32_t i = tid; i < KT * CR; i += 256) {
+                const uint32_t r = i / CR, p = p0 + r;
+                if (p >= last_seen.hi || p < first_seen.lo || !(there >> (r / PART) & 1)) *reinterpret_cast<u32x4*>(v + i * 8) = (u32x4){0, 0, 0, 0};
+            }
+            lh_lds_barrier();
+        }
+        if (!busy || p0 >= wave_last.hi || p0 + KT <= wave_first.lo) continue;
+        lh_f32x16 s[SUB];
+#pragma unroll
+        for (uint32_t u = 0; u < SUB; u++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[u][i] = 0.0f;
+#pragma unroll
+            for (uint32_t c = 0; c < KC; c++)
+                s[u] = product<DT>(*reinterpret_cast<const u32x4*>(K + kat[c % KO] + u * 32 * D + c / KO * KO * 16), qf[c], s[u]);
+        }
+        const bool whole = p0 >= wave_last.lo && p0 + KT <= wave_first.hi && there == 15u;
+        if (!whole)
+#pragma unroll
+            for (uint32_t u = 0; u < SUB; u++)
+#pragma unroll
+                for (uint32_t i = 0; i < 16; i++) {
+                    const uint32_t r = u * 32 + 8 * (i / 4) + 4 * half + (i & 3), p = p0 + r;
+                    if (p < mine.lo || p >= mine.hi || !(there >> (r / PART) & 1)) s[u][i] = -INFINITY;
+                }
+        float mx = -INFINITY;
+#pragma unroll
+        for (uint32_t u = 0; u < SUB; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
+        float ma, mb;
+        lh_pair32(mx, ma, mb);
+        const float nm = fmaxf(m, fmaxf(ma, mb) * scale2);
+        // The reference of the weights follows the maximum only where that has grown 2^8 times: until then they are at most 2^8, which all
+        // types hold as exactly as 1.
+        if (__any(nm > m + 8.0f)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - (nm == -INFINITY ? 0.0f : nm));
+            l *= alpha;
+            m = nm;
+#pragma unroll
+            for (uint32_t d = 0; d < TD; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        u32x4 w[2 * SUB];
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t u = 0; u < SUB; u++)
+#pragma unroll
+            for (uint32_t i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale2, -base)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + 1], scale2, -base));
+                sum += x + y;
+                w[2 * u + i / 8][i / 2 % 4] = pack2<DT>(x, y);
+            }
+        l += sum;
+#pragma unroll
+        for (uint32_t d = 0; d < TD; d++)
+#pragma unroll
+            for (uint32_t k = 0; k < 2 * SUB; k++) {
+                const uint16_t* v = V + vat[d % VO] + k * 16 * D + d / VO * VO * 32;
+                const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)v), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
+                const uint2 xw = __builtin_bit_cast(uint2, x), yw = __builtin_bit_cast(uint2, y);
+                o[d] = product<DT>((u32x4){xw.x, xw.y, yw.x, yw.y}, w[k], o[d]);
+            }
+    }
+    if (!busy) return;
+    const bool alone = part.used == 1;
+    float* rec = alone ? nullptr : a.partial + (((size_t)(t * a.kv_heads + g) * a.splits + z) * 128 + wave * 32) * kRow;
+    bool odd = false;
+#pragma unroll
+    for (uint32_t d = 0; d < TD; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) odd = odd || o[d][i] != o[d][i];
+    if (__any(on && odd)) {
+        for (uint32_t r = 0; r < 32 && wave * 32 + r < tile.count; r++) {
+            const uint32_t pk = tile.row0 + wave * 32 + r, rw = pk / R, hd = g * R + pk - rw * R;
+            const Seen sn = seen_by(a, tile, rw);
+            float sm, sl, sums[(D + 63) / 64];
+            slow_row<DT, D>(a, tile.sequence, (uint64_t)(tile.first + rw) * a.q_ld + (uint64_t)hd * a.dim, g, max(part.begin * KT, sn.lo), min(part.end * KT, sn.hi), lane, sm, sl, sums);
+            const float ref = alone && a.sink ? fmaxf(sm, a.sink[hd] * kLog2e) : sm, zero = ref == -INFINITY ? 0.0f : ref, f = __builtin_amdgcn_exp2f(sm - zero);
+            const float total = sl * f + (alone && a.sink ? __builtin_amdgcn_exp2f(a.sink[hd] * kLog2e - zero) : 0.0f), scale = alone ? (sl == 0.0f ? 0.0f : f / total) : 1.0f;
+            if (rec && lane == 0) { rec[r * kRow + D] = sm == -INFINITY ? 0.0f : sm; rec[r * kRow + D + 1] = sl; }
+#pragma unroll
+            for (int c = 0; c < (D + 63) / 64; c++) {
+                const uint32_t d = lane + 64 * c;
+                if (rec) { if (d < D) rec[r * kRow + d] = sums[c]; }
+                else if (d < a.dim) static_cast<B*>(a.out)[(uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim + d] = element_bits<DT>(sums[c] * scale);
+            }
+        }
+        return;
+    }
+    l = lh_sum32_f(l);
+    if (!on) return;
+    // a lane has columns 32 d + 8 i + 4 half .. + 3 of its row
+    if (rec) {
+        rec += lr * kRow;
+#pragma unroll
+        for (uint32_t d = 0; d < TD; d++)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++)
+                *reinterpret_cast<lh_f32x4*>(rec + 32 * d + 8 * i + 4 * half) = (lh_f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (half == 0) { rec[D] = m == -INFINITY ? 0.0f : m; rec[D + 1] = l; }
+        return;
+    }
+    const float sink = a.sink ? a.sink[head] * kLog2e : -INFINITY, ref = fmaxf(m, sink), zero = ref == -INFINITY ? 0.0f : ref, f = __builtin_amdgcn_exp2f(m - zero);
+    const float inv = l == 0.0f ? 0.0f : f / (l * f + __builtin_amdgcn_exp2f(sink - zero));
+    B* out = static_cast<B*>(a.out) + (uint64_t)(tile.first + row) * a.out_ld + (uint64_t)head * a.dim;
+#pragma unroll
+    for (uint32_t d = 0; d < TD; d++)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t c = 32 * d + 8 * i + 4 * half;
+            const uint2 x = make_uint2(pack2<DT>(o[d][4 * i] * inv, o[d][4 * i + 1] * inv), pack2<DT>(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv));
+            if (a.out_wide) {
+                if (c < a.dim) *reinterpret_cast<uint2*>(out + c) = x;
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) if (c + j < a.dim) out[c + j] = (B)((j < 2 ? x.x : x.y) >> 16 * (j & 1));
+            }
+        }
+}
+// Joins the splits of a tile's rows.  FEW: D / 4 lanes a row, four columns each, the splits one after the other.  Else a workgroup a
+// row: groups of D / 4 lanes take the splits in turn and are added through LDS.
+template <int DT, int D, uint32_t ROWS, uint32_t STEP, bool FEW>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
-    constexpr uint32_t kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS;
-    __shared__ lh_f32x4 sums[256];
+    constexpr uint32_t kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS, PER = FEW ? GROUPS : 1, PARTS = (ROWS + PER - 1) / PER;
+    __shared__ lh_f32x4 sums[FEW ? 1 : 256];
     __shared__ float totals[GROUPS];
-    const uint32_t tid = threadIdx.x, lane = tid & 63;
-    const uint32_t r = blockIdx.x % 16, g = blockIdx.x / 16 % a.kv_heads, t = blockIdx.x / 16 / a.kv_heads;
-    const Tile tile = tile_of<16>(a, t, lane);
-    if (tile.sequence < 0 || r >= tile.count) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, grp = tid / QUADS, c = tid % QUADS * 4;
+    const uint32_t g = blockIdx.x / PARTS % a.kv_heads, t = blockIdx.x / PARTS / a.kv_heads, r = blockIdx.x % PARTS * PER + (FEW ? grp : 0);
+    const Tile tile = tile_of<ROWS>(a, t, lane);
+    if (tile.sequence < 0 || (FEW && grp >= GROUPS) || r >= tile.count) return;
     const uint32_t R = a.heads / a.kv_heads, pk = tile.row0 + r, rw = pk / R, hd = g * R + pk - rw * R;
-    const Part part = part_of(a, seen_by(a, tile, tile.row0 / R).lo, seen_by(a, tile, (tile.row0 + tile.count - 1) / R).hi, 0);
+    const Part part = part_of<STEP>(a, seen_by(a, tile, tile.row0 / R).lo, seen_by(a, tile, (tile.row0 + tile.count - 1) / R).hi, 0);
     if (part.used == 1) return;
-    const float* rec = a.partial + ((size_t)(t * a.kv_heads + g) * a.splits * 16 + r) * kRow;
-    const size_t stride = 16 * kRow;
+    const float* rec = a.partial + ((size_t)(t * a.kv_heads + g) * a.splits * ROWS + r) * kRow;
+    const size_t stride = (size_t)ROWS * kRow;
     float top = -INFINITY;
-    for (uint32_t s = lane; s < part.used; s += 64) if (rec[s * stride + D + 1] != 0.0f) top = fmaxf(top, rec[s * stride + D]);
-    top = lh_group_max(top, 64);
+    if constexpr (FEW) {
+        for (uint32_t s = 0; s < part.used; s++) if (rec[s * stride + D + 1] != 0.0f) top = fmaxf(top, rec[s * stride + D]);
+    } else {
+        for (uint32_t s = lane; s < part.used; s += 64) if (rec[s * stride + D + 1] != 0.0f) top = fmaxf(top, rec[s * stride + D]);
+        top = lh_group_max(top, 64);
+    }
     const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY, ref = fmaxf(top, sink), zero = ref == -INFINITY ? 0.0f : ref;
-    const uint32_t grp = tid / QUADS, c = tid % QUADS * 4;
     lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
     float total = 0.0f;
     if (grp < GROUPS) {
 #pragma unroll 4
-        for (uint32_t s = grp; s < part.used; s += GROUPS) {
+        for (uint32_t s = FEW ? 0 : grp; s < part.used; s += FEW ? 1 : GROUPS) {
             const float* p = rec + s * stride;
             const float l = p[D + 1], f = __builtin_amdgcn_exp2f(p[D] - zero);
             const lh_f32x4 y = *reinterpret_cast<const lh_f32x4*>(p + c);
@@ -400,18 +641,20 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
                 for (int j = 0; j < 4; j++) x[j] += f == 0.0f ? 0.0f : f * y[j];
             }
         }
-        if (c == 0) totals[grp] = total;
     }
-    sums[tid] = x;
-    __syncthreads();
-    if (tid >= QUADS) return;
-    total = 0.0f;
+    if constexpr (!FEW) {
+        if (grp < GROUPS && c == 0) totals[grp] = total;
+        sums[tid] = x;
+        __syncthreads();
+        if (tid >= QUADS) return;
+        total = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < GROUPS; i++) total += totals[i];
+        for (uint32_t i = 0; i < GROUPS; i++) total += totals[i];
 #pragma unroll
-    for (uint32_t i = 1; i < GROUPS; i++)
+        for (uint32_t i = 1; i < GROUPS; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] += sums[i * QUADS + tid][j];
+            for (int j = 0; j < 4; j++) x[j] += sums[i * QUADS + tid][j];
+    }
     const float inv = total == 0.0f ? 0.0f : 1.0f / (total + __builtin_amdgcn_exp2f(sink - zero));
     B* out = static_cast<B*>(a.out) + (uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim;
 #pragma unroll
@@ -420,42 +663,67 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
 
 // How a launch is cut: tiles of all sequences at most, and parts of a tile's positions.
 struct Cut { uint64_t tiles; uint32_t splits, chunk; };
-Cut cut(uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t window) {
+Cut cut(uint32_t tile_rows, uint32_t step, uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t window) {
     const uint32_t R = heads / kv_heads;
     Cut c;
-    c.tiles = std::min<uint64_t>((uint64_t)rows * R / 16 + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + 15) / 16));
-    uint64_t steps = ((uint64_t)max_length + 31) / 32;
-    if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + 16 + 62) / 32);
-    // as many parts as fill the chip, or more where they would be longer than 32 steps; none shorter than 8.  (More steps never make
-    // fewer parts: a workspace is enough for every window.)
-    const uint64_t units = c.tiles * kv_heads, most = (steps + 7) / 8, fewest = (steps + 31) / 32;
-    c.splits = units >= 4096 ? 1u : (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(2048 / units, fewest), most), 1), 512);
+    c.tiles = std::min<uint64_t>((uint64_t)rows * R / tile_rows + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + tile_rows - 1) / tile_rows));
+    uint64_t steps = ((uint64_t)max_length + step - 1) / step;
+    if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + tile_rows + 2 * step - 2) / step);
+    // Few rows: as many parts as fill the chip, or more where they would be longer than 1024 positions; none shorter than 256.  Many rows: what
+    // fills the chip twice.  (More steps never make fewer parts: a workspace is enough for every window.)
+    const uint64_t units = c.tiles * kv_heads, most = (steps * step + 255) / 256, fewest = tile_rows == 16 && units < 4096 ? (steps * step + 1023) / 1024 : 1;
+    const uint64_t fill = tile_rows == 16 ? 2048 / units : 512 / units;
+    c.splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(fill, fewest), most), 1), 512);
     c.chunk = (uint32_t)std::max<uint64_t>((steps + c.splits - 1) / c.splits, 1);
     return c;
 }
+bool takes_tiles(int dtype, uint32_t max_rows, uint32_t heads, uint32_t kv_heads) { return dtype != LH_F32 && (uint64_t)max_rows * (heads / kv_heads) > 16; }
+size_t cut_bytes(const Cut& c, uint32_t tile_rows, uint32_t kv_heads, uint32_t dim) {
+    return c.splits == 1 ? 0 : (size_t)c.tiles * kv_heads * c.splits * tile_rows * (lh_paged_padded_dim(dim) + 4) * 4;
+}
 
+template <int DT, int D, uint32_t ROWS, uint32_t STEP>
+int launch_merge(lh_context* ctx, const PagedArgs& a, const char* op) {
+    constexpr uint32_t per = 256 / (D / 4);
+    // a few splits of many rows: lanes wait for themselves only; else a workgroup a row has more loads on their way
+    if (a.splits <= 8 && (uint64_t)a.tiles * a.kv_heads * ROWS >= 4096)
+        hipLaunchKernelGGL((paged_merge_kernel<DT, D, ROWS, STEP, true>), dim3(a.tiles * a.kv_heads * ((ROWS + per - 1) / per)), dim3(256), 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((paged_merge_kernel<DT, D, ROWS, STEP, false>), dim3(a.tiles * a.kv_heads * ROWS), dim3(256), 0, ctx->stream, a);
+    return lh_check_launch(op);
+}
 template <int DT, int D>
-int launch_rows(lh_context* ctx, const PagedArgs& a, const char* op, uint32_t& launches) {
+int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op, uint32_t& launches) {
+    int r;
+    if constexpr (DT != kF32) if (tiles) {
+        constexpr uint32_t KT = D <= 128 ? 64 : 32;
+        const size_t lds = (size_t)4 * KT * D * 2;
+        if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_tiles_kernel<DT, D>, lds, op)) != LH_OK) return r;
+        hipLaunchKernelGGL((paged_tiles_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
+        launches = 1;
+        if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
+        launches = 2;
+        return launch_merge<DT, D, 128, KT>(ctx, a, op);
+    }
     const size_t lds = (size_t)4 * 16 * (D + 4) * 4;
-    int r = lh_raise_dynamic_lds(ctx, (const void*)paged_rows_kernel<DT, D>, lds, op);
-    if (r != LH_OK) return r;
+    if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_rows_kernel<DT, D>, lds, op)) != LH_OK) return r;
     hipLaunchKernelGGL((paged_rows_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
     launches = 1;
     if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
-    hipLaunchKernelGGL((paged_merge_kernel<DT, D>), dim3(a.tiles * a.kv_heads * 16), dim3(256), 0, ctx->stream, a);
     launches = 2;
-    return lh_check_launch(op);
+    return launch_merge<DT, D, 16, 32>(ctx, a, op);
 }
 template <int DT>
-int launch_rows(lh_context* ctx, const PagedArgs& a, const char* op, uint32_t& launches) {
+int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op, uint32_t& launches) {
     switch (lh_paged_padded_dim(a.dim)) {
-        case 32: return launch_rows<DT, 32>(ctx, a, op, launches);
-        case 64: return launch_rows<DT, 64>(ctx, a, op, launches);
-        case 128: return launch_rows<DT, 128>(ctx, a, op, launches);
-        case 192: return launch_rows<DT, 192>(ctx, a, op, launches);
-        default: return launch_rows<DT, 256>(ctx, a, op, launches);
+        case 32: return launch_rows<DT, 32>(ctx, a, tiles, op, launches);
+        case 64: return launch_rows<DT, 64>(ctx, a, tiles, op, launches);
+        case 128: return launch_rows<DT, 128>(ctx, a, tiles, op, launches);
+        case 192: return launch_rows<DT, 192>(ctx, a, tiles, op, launches);
+        default: return launch_rows<DT, 256>(ctx, a, tiles, op, launches);
     }
 }
+uint32_t tile_step(uint32_t dim) { return dim <= 128 ? 64 : 32; }
 
 }  // namespace
 
@@ -463,8 +731,13 @@ extern "C" {
 
 size_t lh_paged_attention_workspace_bytes(uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t dim) {
     if (kv_heads == 0 || heads == 0 || heads % kv_heads || dim == 0 || dim > 256 || rows == 0 || sequences == 0 || max_rows == 0) return 0;
-    const Cut c = cut(rows, sequences, max_rows, max_length, heads, kv_heads, 0);
-    return c.splits == 1 ? 0 : (size_t)c.tiles * kv_heads * c.splits * 16 * (lh_paged_padded_dim(dim) + 4) * 4;
+    size_t most = 0;                                          // of all types
+    for (int dtype : {LH_BF16, LH_F32}) {
+        const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
+        const uint32_t n = tiles ? 128 : 16;
+        most = std::max(most, cut_bytes(cut(n, tiles ? tile_step(dim) : 32, rows, sequences, max_rows, max_length, heads, kv_heads, 0), n, kv_heads, dim));
+    }
+    return most;
 }
 
 int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer* keys, const lh_buffer* values, lh_buffer* output, int dtype, const lh_buffer* table,
@@ -491,14 +764,15 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
         LH_REQUIRE(((uintptr_t)sink->ptr & 3) == 0, "%s: sink has to begin at 4 bytes", op);
         a.sink = (const float*)sink->ptr;
     }
-    const Cut c = cut(rows, sequences, max_rows, max_length, heads, kv_heads, window);
+    const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
+    const uint32_t tile_rows = tiles ? 128 : 16;
+    const Cut c = cut(tile_rows, tiles ? tile_step(dim) : 32, rows, sequences, max_rows, max_length, heads, kv_heads, window);
     if (c.splits > 1) {
-        const size_t bytes = (size_t)c.tiles * kv_heads * c.splits * 16 * (lh_paged_padded_dim(dim) + 4) * 4;
-        LH_NEED(workspace, bytes, op, "workspace");
+        LH_NEED(workspace, cut_bytes(c, tile_rows, kv_heads, dim), op, "workspace");
         LH_REQUIRE(((uintptr_t)workspace->ptr & 15) == 0, "%s: workspace has to begin at 16 bytes", op);
         a.partial = (float*)workspace->ptr;
     }
-    LH_REQUIRE(c.tiles * kv_heads * std::max(c.splits, 16u) < 0x7FFFFFFFull, "%s: %u rows of %u heads", op, rows, heads);
+    LH_REQUIRE(c.tiles * kv_heads * std::max(c.splits, tile_rows) < 0x7FFFFFFFull, "%s: %u rows of %u heads", op, rows, heads);
     a.q = q->ptr; a.keys = keys->ptr; a.values = values->ptr; a.out = output->ptr;
     a.plan = PagedPlan{(const uint32_t*)table->ptr, (const uint32_t*)starts->ptr, (const uint32_t*)lengths->ptr, rows, sequences, table_ld, pages, (uint32_t)__builtin_ctz(page)};
     a.q_ld = q_ld; a.out_ld = output_ld;
@@ -507,11 +781,12 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     a.tiles = (uint32_t)c.tiles; a.splits = c.splits; a.chunk = c.chunk;
     a.q_wide = (((uintptr_t)a.q | (uint64_t)q_ld * size | (uint64_t)dim * size) & 15) == 0;
     a.out_wide = (((uintptr_t)a.out | (uint64_t)output_ld * size | (uint64_t)dim * size) & 15) == 0;
-    a.scale = scale;
+    a.scale2 = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
+    a.negative = scale < 0.0f; a.nothing = scale == 0.0f;
     uint32_t launches = 0;
-    if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, op, launches);
-    else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, op, launches);
-    else r = launch_rows<kBf16>(batch->ctx, a, op, launches);
+    if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, tiles, op, launches);
+    else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, tiles, op, launches);
+    else r = launch_rows<kBf16>(batch->ctx, a, tiles, op, launches);
     batch->dispatch_count += launches;
     return r;
 }
