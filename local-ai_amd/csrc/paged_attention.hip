@@ -44,9 +44,10 @@ __device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t t, uint32_t
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 64) {
         const uint32_t s = s0 + lane;
-        uint32_t first = 0, all = 0, tiles = 0;
+        uint32_t first = 0, all = 0, tiles = 0, length = 0;
         if (s < a.plan.sequences) {
             first = a.plan.starts[s];
+            length = a.plan.lengths[s];
             const uint32_t end = a.plan.starts[s + 1];
             if (end > first && end <= a.plan.rows) {
                 all = end - first;
@@ -65,7 +66,7 @@ __device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t t, uint32_t
             const uint32_t in = t - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at));
             r.row0 = in * ROWS;
             r.count = min(ROWS, rows - r.row0);
-            r.begin = (int64_t)a.plan.lengths[r.sequence] - n;
+            r.begin = (int64_t)(uint32_t)__builtin_amdgcn_readlane(length, at) - n;
             return r;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
@@ -95,14 +96,21 @@ __device__ __forceinline__ Part part_of(const PagedArgs& a, uint32_t lo, uint32_
 // A wave's view of its sequence's row of the table: 64 entries at a time, one a lane.
 struct Pages {
     const uint32_t* row;
+    uint32_t blocks;                // entries that the wave may need
     uint32_t held, entry;           // entries held .. held + 63
+    uint64_t there;                 // which of them are pages of the pool, or not needed
     __device__ __forceinline__ void load(const PagedPlan& p, uint32_t from, uint32_t lane) {
         held = from;
-        entry = from + lane < p.table_ld ? row[from + lane] : 0xFFFFFFFFu;
+        const uint32_t i = from + lane;
+        entry = i < min(blocks, p.table_ld) ? row[i] : 0xFFFFFFFFu;
+        there = __ballot(i >= blocks || entry < p.pages);
     }
-    __device__ __forceinline__ uint32_t of(const PagedPlan& p, uint32_t block, uint32_t lane) {
-        if (block - held >= 64) load(p, block, lane);
-        return __builtin_amdgcn_readlane(entry, block - held);
+    __device__ __forceinline__ void reach(const PagedPlan& p, uint32_t block, uint32_t lane) { if (block - held >= 64) load(p, block, lane); }
+    // of a block that is held: whether it is there, and its page, or some page
+    __device__ __forceinline__ bool has(uint32_t block) const { return there >> (block - held) & 1; }
+    __device__ __forceinline__ uint32_t of(const PagedPlan& p, uint32_t block) const {
+        const uint32_t pg = __builtin_amdgcn_readlane(entry, block - held);
+        return pg < p.pages ? pg : 0u;
     }
 };
 
@@ -226,7 +234,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
 #pragma unroll
     for (int i = 0; i < DL; i++) o[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
 
-    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, 0, 0};
+    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, (last_seen.hi + (1u << a.plan.shift) - 1) >> a.plan.shift, 0, 0, 0};
     if (begin < end) pages.load(a.plan, (begin * 32) >> a.plan.shift, lane);
     const uint32_t in_page = (1u << a.plan.shift) - 1;
     for (uint32_t b = begin; b < end; b++) {
@@ -234,9 +242,10 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
         bool there[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const uint32_t p = b * 32 + 16 * h, pg = p < last_seen.hi ? pages.of(a.plan, p >> a.plan.shift, lane) : 0xFFFFFFFFu;
-            there[h] = pg < a.plan.pages;
-            base[h] = (((((uint64_t)(there[h] ? pg : 0u) * a.kv_heads + g) << a.plan.shift) + (p & in_page))) * D;
+            const uint32_t p = b * 32 + 16 * h, block = p >> a.plan.shift;
+            pages.reach(a.plan, block, lane);
+            there[h] = pages.has(block);
+            base[h] = (((((uint64_t)pages.of(a.plan, block) * a.kv_heads + g) << a.plan.shift) + (p & in_page))) * D;
         }
         lh_f32x4 s[2];
         uint32_t v[2][4][WIDE ? DL : DL / 2];
@@ -393,17 +402,22 @@ __device__ __forceinline__ lh_f32x16 product(u32x4 x, u32x4 y, lh_f32x16 c) {
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lh_bf16x8, x), __builtin_bit_cast(lh_bf16x8, y), c, 0, 0, 0);
 }
 
+// A key row's pieces are at c ^ key_place(row): rows of 16 pieces fill the banks, shorter ones do so together.
+template <uint32_t PIECES>
+__device__ __forceinline__ constexpr uint32_t key_place(uint32_t row) { return PIECES % 16 == 0 ? row & 15 : PIECES % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3; }
+
 // Many rows, 16-bit types: a workgroup per tile of 128 packed rows, kv head and split.  Each of its four waves has 32 rows, all of them
 // share the steps of KT positions, whose keys and values go from memory to LDS without registers, the next step's while this one is used.
 //   S^T = K Q^T    32 x 32 x 16: a lane has packed row lane & 31 and half of the positions, so maximum and sum are its own registers'
 //   O^T = V^T P^T  the weights are operands where they are; V, in LDS as it is in memory, is read by the transposing ds_read_b64_tr_b16
-// In LDS the 16-byte pieces of a row change places by the row's low bits, so that neither read meets itself in a bank: a key's piece c is
-// at c ^ (row & 7), a value's at c ^ 4 (row & 3).
+// In LDS the 16-byte pieces of a row change places by the row's low bits, so that neither read meets itself in one of the 64 banks: of
+// 16 neighbouring key rows the same piece is in 16 places (key_place), of four value rows the same four pieces in four.
 template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void paged_tiles_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
     constexpr uint32_t KT = D <= 128 ? 64 : 32, SUB = KT / 32, KC = D / 16, TD = D / 32, CR = D / 8, PART = KT / 4, LOADS = PART * D / 512, kRow = D + 4;
     constexpr uint32_t VSWAP = CR % 16 == 0 ? 3 : CR % 8 == 0 ? 1 : 0;
+    constexpr bool AHEAD = D <= 128;                          // (more columns leave no registers for it)
     extern __shared__ __align__(16) uint16_t stage[];         // [2][keys, values][KT][D]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, lr = lane & 31;
     const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = a.tiles - 1 - blockIdx.x / a.kv_heads / a.splits;    // long tiles first
@@ -428,23 +442,24 @@ __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(const PagedArgs a) 
     uint32_t kfrom[LOADS], vfrom[LOADS];
 #pragma unroll
     for (uint32_t j = 0; j < LOADS; j++) {
-        const uint32_t id = j * 64 + lane, r = id / CR, c = id % CR, k = CR >= 8 ? (wave * PART + r) & 7 : ((wave * PART + r) >> 1) & 3;
-        kfrom[j] = (r * D + (c ^ k) * 8) * 2;
+        const uint32_t id = j * 64 + lane, r = id / CR, c = id % CR;
+        kfrom[j] = (r * D + (c ^ key_place<CR>(wave * PART + r)) * 8) * 2;
         vfrom[j] = (r * D + (c ^ (((wave * PART + r) & VSWAP) << 2)) * 8) * 2;
     }
-    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, 0, 0};
+    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, (last_seen.hi + (1u << a.plan.shift) - 1) >> a.plan.shift, 0, 0, 0};
     const uint32_t in_page = (1u << a.plan.shift) - 1;
     if (part.begin < part.end) pages.load(a.plan, (part.begin * KT) >> a.plan.shift, lane);
     // Requests step b into buffer `at`; returns which quarters of it are there.
     auto request = [&](uint32_t b, uint32_t at) __attribute__((always_inline)) {
-        uint32_t there = 0, own = 0;
+        const uint32_t block = (b * KT + wave * PART) >> a.plan.shift, first = (b * KT) >> a.plan.shift;
+        if (first - pages.held > 60) pages.load(a.plan, first, lane);             // (a step has four at most)
+        uint32_t there = 15;
+        if (pages.there != ~0ull) {
+            there = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            const uint32_t p = b * KT + i * PART, pg = p < last_seen.hi ? pages.of(a.plan, p >> a.plan.shift, lane) : 0xFFFFFFFFu;
-            if (pg < a.plan.pages) there |= 1u << i;
-            if (i == wave) own = pg < a.plan.pages ? pg : 0u;
+            for (uint32_t i = 0; i < 4; i++) there |= (uint32_t)pages.has((b * KT + i * PART) >> a.plan.shift) << i;
         }
-        const uint64_t base = ((((uint64_t)own * a.kv_heads + g) << a.plan.shift) + ((b * KT + wave * PART) & in_page)) * D;
+        const uint64_t base = ((((uint64_t)pages.of(a.plan, block) * a.kv_heads + g) << a.plan.shift) + ((b * KT + wave * PART) & in_page)) * D;
         const B *K = static_cast<const B*>(a.keys) + base, *V = static_cast<const B*>(a.values) + base;
         const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)(stage + (at * 2 * KT + wave * PART) * D));
 #pragma unroll
@@ -454,10 +469,10 @@ __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(const PagedArgs a) 
         return there;
     };
     // where a lane reads operands, in values: of keys row lr, of values row 4 half + (lane & 15) / 4
-    constexpr uint32_t KO = CR >= 8 ? 4 : 2, VO = VSWAP == 3 ? 4 : VSWAP == 1 ? 2 : 1;
+    constexpr uint32_t KO = CR % 16 == 0 ? 8 : CR % 8 == 0 ? 4 : 2, VO = VSWAP == 3 ? 4 : VSWAP == 1 ? 2 : 1;
     uint32_t kat[KO], vat[VO];
 #pragma unroll
-    for (uint32_t c = 0; c < KO; c++) kat[c] = lr * D + ((c * 2 + half) ^ (CR >= 8 ? lr & 7 : (lr >> 1) & 3)) * 8;
+    for (uint32_t c = 0; c < KO; c++) kat[c] = lr * D + ((c * 2 + half) ^ key_place<CR>(lr)) * 8;
 #pragma unroll
     for (uint32_t c = 0; c < VO; c++) {
         const uint32_t i = lane & 15, r = 4 * half + (i >> 2), piece = c * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
@@ -487,14 +502,33 @@ __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(const PagedArgs a) 
             lh_lds_barrier();
         }
         if (!busy || p0 >= wave_last.hi || p0 + KT <= wave_first.lo) continue;
+        // AHEAD: operands are requested a group of products ahead: 32 positions of keys, 32 columns of values
         lh_f32x16 s[SUB];
+        u32x4 kf[2][KC], vf[2][2 * SUB];
+        auto keys_of = [&](uint32_t u, u32x4 (&x)[KC]) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t c = 0; c < KC; c++) x[c] = *reinterpret_cast<const u32x4*>(K + kat[c % KO] + u * 32 * D + c / KO * KO * 16);
+        };
+        auto values_of = [&](uint32_t d, u32x4 (&x)[2 * SUB]) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t k = 0; k < 2 * SUB; k++) {
+                const uint16_t* v = V + vat[d % VO] + k * 16 * D + d / VO * VO * 32;
+                const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)v));
+                const uint2 z = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D)));
+                x[k] = (u32x4){y.x, y.y, z.x, z.y};
+            }
+        };
+        if (AHEAD) keys_of(0, kf[0]);
 #pragma unroll
         for (uint32_t u = 0; u < SUB; u++) {
+            if (!AHEAD) keys_of(u, kf[u & 1]);
+            else if (u + 1 < SUB) keys_of(u + 1, kf[(u + 1) & 1]);
+            else values_of(0, vf[0]);
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 16; i++) s[u][i] = 0.0f;
 #pragma unroll
-            for (uint32_t c = 0; c < KC; c++)
-                s[u] = product<DT>(*reinterpret_cast<const u32x4*>(K + kat[c % KO] + u * 32 * D + c / KO * KO * 16), qf[c], s[u]);
+            for (uint32_t c = 0; c < KC; c++) s[u] = product<DT>(kf[u & 1][c], qf[c], s[u]);
         }
         const bool whole = p0 >= wave_last.lo && p0 + KT <= wave_first.hi && there == 15u;
         if (!whole)
@@ -537,14 +571,13 @@ __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(const PagedArgs a) 
             }
         l += sum;
 #pragma unroll
-        for (uint32_t d = 0; d < TD; d++)
+        for (uint32_t d = 0; d < TD; d++) {
+            if (!AHEAD) values_of(d, vf[d & 1]);
+            else if (d + 1 < TD) values_of(d + 1, vf[(d + 1) & 1]);
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (uint32_t k = 0; k < 2 * SUB; k++) {
-                const uint16_t* v = V + vat[d % VO] + k * 16 * D + d / VO * VO * 32;
-                const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)v), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
-                const uint2 xw = __builtin_bit_cast(uint2, x), yw = __builtin_bit_cast(uint2, y);
-                o[d] = product<DT>((u32x4){xw.x, xw.y, yw.x, yw.y}, w[k], o[d]);
-            }
+            for (uint32_t k = 0; k < 2 * SUB; k++) o[d] = product<DT>(vf[d & 1][k], w[k], o[d]);
+        }
     }
     if (!busy) return;
     const bool alone = part.used == 1;
@@ -602,14 +635,15 @@ __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(const PagedArgs a) 
             }
         }
 }
-// Joins the splits of a tile's rows.  FEW: D / 4 lanes a row, four columns each, the splits one after the other.  Else a workgroup a
-// row: groups of D / 4 lanes take the splits in turn and are added through LDS.
+// Joins the splits of a tile's rows: D / 4 lanes take a split's sums, four columns each, eight splits on their way at a time, and keep a
+// running maximum of what they have seen.  FEW: these lanes are all that a row has.  Else a workgroup a row, whose
+// groups of lanes take the splits in turn and meet in LDS.
 template <int DT, int D, uint32_t ROWS, uint32_t STEP, bool FEW>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
-    constexpr uint32_t kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS, PER = FEW ? GROUPS : 1, PARTS = (ROWS + PER - 1) / PER;
+    constexpr uint32_t kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS, PER = FEW ? GROUPS : 1, PARTS = (ROWS + PER - 1) / PER, BATCH = 8;
     __shared__ lh_f32x4 sums[FEW ? 1 : 256];
-    __shared__ float totals[GROUPS];
+    __shared__ float2 totals[GROUPS];
     const uint32_t tid = threadIdx.x, lane = tid & 63, grp = tid / QUADS, c = tid % QUADS * 4;
     const uint32_t g = blockIdx.x / PARTS % a.kv_heads, t = blockIdx.x / PARTS / a.kv_heads, r = blockIdx.x % PARTS * PER + (FEW ? grp : 0);
     const Tile tile = tile_of<ROWS>(a, t, lane);
@@ -619,43 +653,61 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     if (part.used == 1) return;
     const float* rec = a.partial + ((size_t)(t * a.kv_heads + g) * a.splits * ROWS + r) * kRow;
     const size_t stride = (size_t)ROWS * kRow;
-    float top = -INFINITY;
-    if constexpr (FEW) {
-        for (uint32_t s = 0; s < part.used; s++) if (rec[s * stride + D + 1] != 0.0f) top = fmaxf(top, rec[s * stride + D]);
-    } else {
-        for (uint32_t s = lane; s < part.used; s += 64) if (rec[s * stride + D + 1] != 0.0f) top = fmaxf(top, rec[s * stride + D]);
-        top = lh_group_max(top, 64);
-    }
-    const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY, ref = fmaxf(top, sink), zero = ref == -INFINITY ? 0.0f : ref;
+    const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY;
     lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
-    float total = 0.0f;
-    if (grp < GROUPS) {
-#pragma unroll 4
-        for (uint32_t s = FEW ? 0 : grp; s < part.used; s += FEW ? 1 : GROUPS) {
-            const float* p = rec + s * stride;
-            const float l = p[D + 1], f = __builtin_amdgcn_exp2f(p[D] - zero);
-            const lh_f32x4 y = *reinterpret_cast<const lh_f32x4*>(p + c);
-            if (l != 0.0f) {
-                total += f * l;
+    float m = -INFINITY, l = 0.0f;
+    const uint32_t each = FEW ? 1 : GROUPS;
+    for (uint32_t s0 = FEW ? 0 : grp; s0 < part.used && grp < GROUPS; s0 += each * BATCH) {
+        lh_f32x4 y[BATCH];
+        float2 st[BATCH];
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[j] += f == 0.0f ? 0.0f : f * y[j];
-            }
+        for (uint32_t i = 0; i < BATCH; i++) {
+            const float* p = rec + min(s0 + i * each, part.used - 1) * stride;
+            y[i] = *reinterpret_cast<const lh_f32x4*>(p + c);
+            st[i] = *reinterpret_cast<const float2*>(p + D);
+        }
+        float nm = m;
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; i++) {
+            if (s0 + i * each >= part.used || st[i].y == 0.0f) { st[i] = make_float2(-INFINITY, 0.0f); y[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f}; }    // nothing seen there
+            nm = fmaxf(nm, st[i].x);
+        }
+        const float zero = nm == -INFINITY ? 0.0f : nm, before = __builtin_amdgcn_exp2f(m - zero);
+        m = nm;
+        l *= before;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] *= before;
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; i++) {
+            const float f = __builtin_amdgcn_exp2f(st[i].x - zero);
+            l += f * st[i].y;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] += f * y[i][j];
         }
     }
     if constexpr (!FEW) {
-        if (grp < GROUPS && c == 0) totals[grp] = total;
         sums[tid] = x;
+        if (c == 0 && grp < GROUPS) totals[grp] = make_float2(m, l);
         __syncthreads();
         if (tid >= QUADS) return;
-        total = 0.0f;
+        float top = -INFINITY;
 #pragma unroll
-        for (uint32_t i = 0; i < GROUPS; i++) total += totals[i];
+        for (uint32_t i = 0; i < GROUPS; i++) top = fmaxf(top, totals[i].x);
+        m = top;
+        const float zero = m == -INFINITY ? 0.0f : m;
+        l = 0.0f;
+        x = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (uint32_t i = 1; i < GROUPS; i++)
+        for (uint32_t i = 0; i < GROUPS; i++) {
+            const float f = __builtin_amdgcn_exp2f(totals[i].x - zero);
+            const lh_f32x4 y = sums[i * QUADS + tid];
+            l += f * totals[i].y;
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] += sums[i * QUADS + tid][j];
+            for (int j = 0; j < 4; j++) x[j] += f * y[j];
+        }
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / (total + __builtin_amdgcn_exp2f(sink - zero));
+    const float ref = fmaxf(m, sink), zero = ref == -INFINITY ? 0.0f : ref, f = __builtin_amdgcn_exp2f(m - zero);
+    const float inv = l == 0.0f ? 0.0f : f / (l * f + __builtin_amdgcn_exp2f(sink - zero));
     B* out = static_cast<B*>(a.out) + (uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim;
 #pragma unroll
     for (int j = 0; j < 4; j++) if (c + j < a.dim) out[c + j] = element_bits<DT>(x[j] * inv);
@@ -669,9 +721,9 @@ Cut cut(uint32_t tile_rows, uint32_t step, uint32_t rows, uint32_t sequences, ui
     c.tiles = std::min<uint64_t>((uint64_t)rows * R / tile_rows + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + tile_rows - 1) / tile_rows));
     uint64_t steps = ((uint64_t)max_length + step - 1) / step;
     if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + tile_rows + 2 * step - 2) / step);
-    // Few rows: as many parts as fill the chip, or more where they would be longer than 1024 positions; none shorter than 256.  Many rows: what
+    // Few rows: as many parts as fill the chip, or more where they would be longer than 1024 positions; none shorter than 512.  Many rows: what
     // fills the chip twice.  (More steps never make fewer parts: a workspace is enough for every window.)
-    const uint64_t units = c.tiles * kv_heads, most = (steps * step + 255) / 256, fewest = tile_rows == 16 && units < 4096 ? (steps * step + 1023) / 1024 : 1;
+    const uint64_t units = c.tiles * kv_heads, most = steps * step / (tile_rows == 16 ? 512 : 256), fewest = tile_rows == 16 && units < 4096 ? (steps * step + 1023) / 1024 : 1;
     const uint64_t fill = tile_rows == 16 ? 2048 / units : 512 / units;
     c.splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(fill, fewest), most), 1), 512);
     c.chunk = (uint32_t)std::max<uint64_t>((steps + c.splits - 1) / c.splits, 1);
@@ -685,8 +737,8 @@ size_t cut_bytes(const Cut& c, uint32_t tile_rows, uint32_t kv_heads, uint32_t d
 template <int DT, int D, uint32_t ROWS, uint32_t STEP>
 int launch_merge(lh_context* ctx, const PagedArgs& a, const char* op) {
     constexpr uint32_t per = 256 / (D / 4);
-    // a few splits of many rows: lanes wait for themselves only; else a workgroup a row has more loads on their way
-    if (a.splits <= 8 && (uint64_t)a.tiles * a.kv_heads * ROWS >= 4096)
+    // up to eight splits are on their way at once; more of them, too, where the rows fill the chip without
+    if (a.splits <= 8 || (a.splits <= 32 && (uint64_t)a.tiles * a.kv_heads * ROWS >= 4096))
         hipLaunchKernelGGL((paged_merge_kernel<DT, D, ROWS, STEP, true>), dim3(a.tiles * a.kv_heads * ((ROWS + per - 1) / per)), dim3(256), 0, ctx->stream, a);
     else
         hipLaunchKernelGGL((paged_merge_kernel<DT, D, ROWS, STEP, false>), dim3(a.tiles * a.kv_heads * ROWS), dim3(256), 0, ctx->stream, a);
