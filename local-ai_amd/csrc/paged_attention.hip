@@ -25,6 +25,7 @@ struct PagedArgs {
     uint64_t q_ld, out_ld;
     uint32_t max_rows, heads, kv_heads, dim, window, capacity;     // capacity: positions from there on are not seen
     uint32_t tiles, splits, chunk;                                 // chunk: steps that a split takes at least
+    uint32_t stream;                                               // the caches are more than stays near the chip
     uint32_t q_wide, out_wide;                                     // rows, heads and their ends at 16 bytes
     float scale2;              // of the products, in powers of two; > 0
     uint32_t negative, nothing;                                    // the scale is below zero, or zero: in the queries
@@ -129,12 +130,17 @@ __device__ __forceinline__ float low(uint32_t x) { return element_value<DT>((ele
 template <int DT>
 __device__ __forceinline__ float high(uint32_t x) { return element_value<DT>((element_t<DT>)(x >> 16)); }
 
+template <bool STREAM>
+__device__ __forceinline__ u32x4 load16(const void* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(static_cast<const u32x4*>(p));
+    else return *static_cast<const u32x4*>(p);
+}
 // N dwords from an address that is a multiple of their largest power of two
-template <int N>
+template <bool STREAM, int N>
 __device__ __forceinline__ void load_words(const void* p, uint32_t (&x)[N]) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) { const u32x4 v = *reinterpret_cast<const u32x4*>((const char*)p + 4 * i); x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w; }
+        for (int i = 0; i < N; i += 4) { const u32x4 v = load16<STREAM>((const char*)p + 4 * i); x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w; }
     } else if constexpr (N % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) { const uint2 v = *reinterpret_cast<const uint2*>((const char*)p + 4 * i); x[i] = v.x; x[i + 1] = v.y; }
@@ -206,11 +212,12 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint6
 //   O^T = V^T P^T  the weights are operands where they are; of V a lane loads D / 16 neighbouring columns of its eight positions, and
 //                  pairs of positions are put together in registers, a column per product: no LDS on the way
 // Weights of 16 bits are two terms, what the first leaves being the second.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
+// The next step's keys are requested when this one's are used, its values likewise.  STREAM: with the hint that nothing is read again.
+template <int DT, int D, bool STREAM>
+__global__ __launch_bounds__(256, DT == kF32 ? 1 : D <= 128 ? 3 : 2) void paged_rows_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
-    constexpr bool WIDE = DT == kF32;
-    constexpr int DL = D / 16, kRow = D + 4, KC = WIDE ? D / 16 : D / 32;
+    constexpr bool WIDE = DT == kF32, AHEAD = !WIDE || D <= 64;      // (wider rows of 32 bits leave no registers for it)
+    constexpr int DL = D / 16, kRow = D + 4, KC = WIDE ? D / 16 : D / 32, VW = WIDE ? DL : DL / 2;
     extern __shared__ __align__(16) float slab[];             // [4 waves][16][kRow]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gr = lane >> 4, lr = lane & 15;
     const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = blockIdx.x / a.kv_heads / a.splits;
@@ -237,39 +244,56 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
     Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, (last_seen.hi + (1u << a.plan.shift) - 1) >> a.plan.shift, 0, 0, 0};
     if (begin < end) pages.load(a.plan, (begin * 32) >> a.plan.shift, lane);
     const uint32_t in_page = (1u << a.plan.shift) - 1;
-    for (uint32_t b = begin; b < end; b++) {
-        uint64_t base[2];                                     // of the page's rows for this kv head, from the half's first slot on
-        bool there[2];
+    // Where step b's halves stand: the page's rows for this kv head, from the half's first slot on.
+    uint64_t base[2];
+    bool next_there[2];
+    auto locate = [&](uint32_t b) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint32_t p = b * 32 + 16 * h, block = p >> a.plan.shift;
             pages.reach(a.plan, block, lane);
-            there[h] = pages.has(block);
+            next_there[h] = pages.has(block);
             base[h] = (((((uint64_t)pages.of(a.plan, block) * a.kv_heads + g) << a.plan.shift) + (p & in_page))) * D;
         }
-        lh_f32x4 s[2];
-        uint32_t v[2][4][WIDE ? DL : DL / 2];
+    };
+    u32x4 kf[2][KC];
+    uint32_t v[2][4][VW];
+    auto load_keys = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const B* K = static_cast<const B*>(a.keys) + base[h] + lr * D + gr * (WIDE ? 4 : 8);
-            u32x4 kf[KC];
 #pragma unroll
-            for (int c = 0; c < KC; c++) kf[c] = *reinterpret_cast<const u32x4*>(K + c * (WIDE ? 16 : 32));
+            for (int c = 0; c < KC; c++) kf[h][c] = load16<STREAM>(K + c * (WIDE ? 16 : 32));
+        }
+    };
+    auto load_values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
             const B* V = static_cast<const B*>(a.values) + base[h] + gr * 4 * D + lr * DL;
 #pragma unroll
-            for (int j = 0; j < 4; j++) load_words(V + j * D, v[h][j]);
+            for (int j = 0; j < 4; j++) load_words<STREAM>(V + j * D, v[h][j]);
+        }
+    };
+    if (AHEAD && begin < end) { locate(begin); load_keys(); load_values(); }
+    for (uint32_t b = begin; b < end; b++) {
+        if (!AHEAD) { locate(b); load_keys(); load_values(); }
+        const bool there[2] = {next_there[0], next_there[1]};
+        lh_f32x4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
             s[h] = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < KC; c++) {
                 if constexpr (WIDE) {
-                    const lh_f32x4 x = __builtin_bit_cast(lh_f32x4, kf[c]), y = __builtin_bit_cast(lh_f32x4, qf[c]);
+                    const lh_f32x4 x = __builtin_bit_cast(lh_f32x4, kf[h][c]), y = __builtin_bit_cast(lh_f32x4, qf[c]);
 #pragma unroll
                     for (int j = 0; j < 4; j++) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], s[h], 0, 0, 0);
                 } else {
-                    s[h] = product<DT>(kf[c], qf[c], s[h]);
+                    s[h] = product<DT>(kf[h][c], qf[c], s[h]);
                 }
             }
         }
+        if (AHEAD && b + 1 < end) { locate(b + 1); load_keys(); }
         float p[8], mx = -INFINITY;
         const bool whole = b * 32 >= last_seen.lo && b * 32 + 32 <= first_seen.hi && there[0] && there[1];
 #pragma unroll
@@ -280,7 +304,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
                 if (at < mine.lo || at >= mine.hi || !there[i >> 2]) p[i] = -INFINITY;
                 if (at >= last_seen.hi || at < first_seen.lo || !there[i >> 2]) {      // seen by none: may be anything
 #pragma unroll
-                    for (int e = 0; e < (WIDE ? DL : DL / 2); e++) v[i >> 2][i & 3][e] = 0;
+                    for (int e = 0; e < VW; e++) v[i >> 2][i & 3][e] = 0;
                 }
             }
             mx = fmaxf(mx, p[i]);
@@ -317,6 +341,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(const PagedArgs a) {
                 o[i] = product<DT>(x, lo, o[i]);
             }
         }
+        if (AHEAD && b + 1 < end) load_values();
     }
     // The wave's results: row lr, columns (4 gr + j) DL + i.
     float* own = slab + wave * 16 * kRow;
@@ -487,8 +512,9 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     uint32_t next_there = part.begin < part.end ? request(part.begin, 0) : 0u;
-    for (uint32_t b = part.begin; b < part.end; b++) {
-        const uint32_t at = (b - part.begin) & 1, there = next_there, p0 = b * KT;
+    auto step = [&](uint32_t b, auto buffer) __attribute__((always_inline)) {
+        constexpr uint32_t at = decltype(buffer)::value;      // a constant: it goes into the reads' offsets
+        const uint32_t there = next_there, p0 = b * KT;
         wait_for_loads();
         __syncthreads();                                      // the step is there, and nobody reads the other buffer any more
         if (b + 1 < part.end) next_there = request(b + 1, at ^ 1);
@@ -501,7 +527,7 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
             }
             lh_lds_barrier();
         }
-        if (!busy || p0 >= wave_last.hi || p0 + KT <= wave_first.lo) continue;
+        if (!busy || p0 >= wave_last.hi || p0 + KT <= wave_first.lo) return;
         // AHEAD: operands are requested a group of products ahead: 32 positions of keys, 32 columns of values
         lh_f32x16 s[SUB];
         u32x4 kf[2][KC], vf[2][2 * SUB];
@@ -527,8 +553,10 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
             if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 16; i++) s[u][i] = 0.0f;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (uint32_t c = 0; c < KC; c++) s[u] = product<DT>(kf[u & 1][c], qf[c], s[u]);
+            __builtin_amdgcn_s_setprio(0);
         }
         const bool whole = p0 >= wave_last.lo && p0 + KT <= wave_first.hi && there == 15u;
         if (!whole)
@@ -572,12 +600,18 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
         l += sum;
 #pragma unroll
         for (uint32_t d = 0; d < TD; d++) {
+            if (d == 0) __builtin_amdgcn_s_setprio(1);
             if (!AHEAD) values_of(d, vf[d & 1]);
             else if (d + 1 < TD) values_of(d + 1, vf[(d + 1) & 1]);
             if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (uint32_t k = 0; k < 2 * SUB; k++) o[d] = product<DT>(vf[d & 1][k], w[k], o[d]);
+            if (d + 1 == TD) __builtin_amdgcn_s_setprio(0);
         }
+    };
+    for (uint32_t b = part.begin; b < part.end; b += 2) {
+        step(b, std::integral_constant<uint32_t, 0>());
+        if (b + 1 < part.end) step(b + 1, std::integral_constant<uint32_t, 1>());
     }
     if (!busy) return;
     const bool alone = part.used == 1;
@@ -721,9 +755,9 @@ Cut cut(uint32_t tile_rows, uint32_t step, uint32_t rows, uint32_t sequences, ui
     c.tiles = std::min<uint64_t>((uint64_t)rows * R / tile_rows + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + tile_rows - 1) / tile_rows));
     uint64_t steps = ((uint64_t)max_length + step - 1) / step;
     if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + tile_rows + 2 * step - 2) / step);
-    // Few rows: as many parts as fill the chip, or more where they would be longer than 1024 positions; none shorter than 512.  Many rows: what
+    // Few rows: as many parts as fill the chip, or more where they would be longer than 2048 positions; none shorter than 512.  Many rows: what
     // fills the chip twice.  (More steps never make fewer parts: a workspace is enough for every window.)
-    const uint64_t units = c.tiles * kv_heads, most = steps * step / (tile_rows == 16 ? 512 : 256), fewest = tile_rows == 16 && units < 4096 ? (steps * step + 1023) / 1024 : 1;
+    const uint64_t units = c.tiles * kv_heads, most = steps * step / (tile_rows == 16 ? 512 : 256), fewest = tile_rows == 16 && units < 4096 ? (steps * step + 2047) / 2048 : 1;
     const uint64_t fill = tile_rows == 16 ? 2048 / units : 512 / units;
     c.splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(fill, fewest), most), 1), 512);
     c.chunk = (uint32_t)std::max<uint64_t>((steps + c.splits - 1) / c.splits, 1);
@@ -758,8 +792,9 @@ int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op,
         return launch_merge<DT, D, 128, KT>(ctx, a, op);
     }
     const size_t lds = (size_t)4 * 16 * (D + 4) * 4;
-    if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_rows_kernel<DT, D>, lds, op)) != LH_OK) return r;
-    hipLaunchKernelGGL((paged_rows_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
+    const auto rows_kernel = a.stream ? paged_rows_kernel<DT, D, true> : paged_rows_kernel<DT, D, false>;
+    if ((r = lh_raise_dynamic_lds(ctx, (const void*)rows_kernel, lds, op)) != LH_OK) return r;
+    hipLaunchKernelGGL(rows_kernel, dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
     launches = 1;
     if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
     launches = 2;
@@ -835,6 +870,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     a.out_wide = (((uintptr_t)a.out | (uint64_t)output_ld * size | (uint64_t)dim * size) & 15) == 0;
     a.scale2 = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
     a.negative = scale < 0.0f; a.nothing = scale == 0.0f;
+    a.stream = (uint64_t)sequences * max_length * kv_heads * 2 * lh_paged_padded_dim(dim) * size > (256ull << 20);
     uint32_t launches = 0;
     if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, tiles, op, launches);
     else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, tiles, op, launches);
