@@ -20,7 +20,7 @@ struct PagedArgs {
     const void *q, *keys, *values;
     void* out;
     const float* sink;         // [heads], may be null
-    float* partial;            // records [tile][kv head][split][row of the tile][D + 4]: unnormalised sums, maximum, sum of weights
+    float* partial;            // records [tile][kv head][split] of (D + 4) values a row: unnormalised sums, maximum, sum of weights
     PagedPlan plan;
     uint64_t q_ld, out_ld;
     uint32_t max_rows, heads, kv_heads, dim, window, capacity;     // capacity: positions from there on are not seen
@@ -30,6 +30,17 @@ struct PagedArgs {
     float scale2;              // of the products, in powers of two; > 0
     uint32_t negative, nothing;                                    // the scale is below zero, or zero: in the queries
 };
+
+// The sum over this lane and the ones before it.
+__device__ __forceinline__ uint32_t sum_up_to(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);      // row_shr:1, 2, 4, 8, row_bcast:15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xE, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xC, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 
 // A tile of a sequence: its rows row0 .. row0 + count - 1 of the packed ones.
 struct Tile {
@@ -55,9 +66,7 @@ __device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t t, uint32_t
                 tiles = (uint32_t)(((uint64_t)min(all, a.max_rows) * R + ROWS - 1) / ROWS);
             }
         }
-        uint32_t sum = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) { const uint32_t x = __shfl_up(sum, d); if (lane >= (uint32_t)d) sum += x; }
+        const uint32_t sum = sum_up_to(tiles);
         const uint64_t behind = __ballot(before + sum > t);
         if (behind) {
             const int at = __builtin_ctzll(behind);
@@ -150,24 +159,35 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t (&x)[N]) {
     }
 }
 
-// 16 bytes of a query from column d on, zeros behind its end; the scale's sign goes into it.
-template <int DT>
-__device__ __forceinline__ u32x4 query_words(const PagedArgs& a, uint64_t q_at, uint32_t d, bool on) {
+// A lane's N pieces of 16 bytes of the query at q_at, the first at column d, `apart` columns from one to the next; zeros behind the head's
+// end and where `on` is false (q_at is a query's all the same).  The scale's sign goes into them.  All loads are on their way together.
+template <int DT, int N>
+__device__ __forceinline__ void load_query(const PagedArgs& a, uint64_t q_at, uint32_t d, uint32_t apart, bool on, u32x4 (&x)[N]) {
     typedef element_t<DT> B;
     constexpr uint32_t n = 16 / sizeof(B);
-    u32x4 x = {0, 0, 0, 0};
-    if (!on || a.nothing) return x;
+    const B* q = static_cast<const B*>(a.q) + q_at;
     if (a.q_wide) {
-        if (d < a.dim) x = *reinterpret_cast<const u32x4*>(static_cast<const B*>(a.q) + q_at + d);
+#pragma unroll
+        for (int c = 0; c < N; c++) x[c] = *reinterpret_cast<const u32x4*>(q + (d + c * apart < a.dim ? d + c * apart : 0u));
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < n; i++)
-            if (d + i < a.dim) x[i * sizeof(B) / 4] |= (uint32_t)static_cast<const B*>(a.q)[q_at + d + i] << (DT == kF32 ? 0 : 16 * (i & 1));
-    }
-    if (a.negative)
+        for (int c = 0; c < N; c++) {
+            B e[n];
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] ^= DT == kF32 ? 0x80000000u : 0x80008000u;
-    return x;
+            for (uint32_t i = 0; i < n; i++) e[i] = q[min(d + c * apart + i, a.dim - 1)];
+#pragma unroll
+            for (uint32_t i = 0; i < n; i++) if (d + c * apart + i >= a.dim) e[i] = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) x[c][i] = DT == kF32 ? (uint32_t)e[i * n / 4] : (uint32_t)e[i * n / 4] | (uint32_t)e[(i * n + n / 2) / 4] << 16;
+        }
+    }
+    const uint32_t sign = !a.negative ? 0u : DT == kF32 ? 0x80000000u : 0x80008000u;
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+        const bool in = on && !a.nothing && (!a.q_wide || d + c * apart < a.dim);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[c][i] = in ? x[c][i] ^ sign : 0u;
+    }
 }
 
 // One packed row over positions begin .. end - 1, by one wave and value by value: what takes the place of the matrix instructions where a
@@ -214,7 +234,7 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint6
 // Weights of 16 bits are two terms, what the first leaves being the second.
 // The next step's keys are requested when this one's are used, its values likewise.  STREAM: with the hint that nothing is read again.
 template <int DT, int D, bool STREAM>
-__global__ __launch_bounds__(256, DT == kF32 ? 1 : D <= 128 ? 3 : 2) void paged_rows_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3 : 2) void paged_rows_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
     constexpr bool WIDE = DT == kF32, AHEAD = !WIDE || D <= 64;      // (wider rows of 32 bits leave no registers for it)
     constexpr int DL = D / 16, kRow = D + 4, KC = WIDE ? D / 16 : D / 32, VW = WIDE ? DL : DL / 2;
@@ -223,18 +243,17 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : D <= 128 ? 3 : 2) void paged_
     const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = blockIdx.x / a.kv_heads / a.splits;
     const Tile tile = tile_of<16>(a, t, lane);
     if (tile.sequence < 0) return;
-    const uint32_t R = a.heads / a.kv_heads, packed = tile.row0 + lr, row = packed / R, head = g * R + packed - row * R;
+    const uint32_t R = a.heads / a.kv_heads, packed = tile.row0 + min(lr, tile.count - 1), row = packed / R, head = g * R + packed - row * R;
     const bool on = lr < tile.count;
     const uint32_t last_row = (tile.row0 + tile.count - 1) / R, first_row = tile.row0 / R;
-    const Seen mine = seen_by(a, tile, min(row, last_row)), first_seen = seen_by(a, tile, first_row), last_seen = seen_by(a, tile, last_row);
+    const Seen mine = seen_by(a, tile, row), first_seen = seen_by(a, tile, first_row), last_seen = seen_by(a, tile, last_row);
     const Part part = part_of<32>(a, first_seen.lo, last_seen.hi, z);
     if (z >= part.used) return;
     const uint32_t per = (part.end - part.begin + 3) / 4, begin = min(part.begin + wave * per, part.end), end = min(begin + per, part.end);
     const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
 
     u32x4 qf[KC];
-#pragma unroll
-    for (int c = 0; c < KC; c++) qf[c] = query_words<DT>(a, q_at, (c * 4 + gr) * (WIDE ? 4 : 8), on);
+    load_query<DT>(a, q_at, gr * (WIDE ? 4 : 8), WIDE ? 16 : 32, on, qf);
     const float scale2 = a.scale2;
     float m = -INFINITY, l = 0.0f;
     lh_f32x4 o[DL];
@@ -409,8 +428,9 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : D <= 128 ? 3 : 2) void paged_
 
 typedef float lh_f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 // 16 bytes a lane from base + from straight to LDS, lane by lane from byte `to` on (the same in all lanes).  No registers are written, so
 // nothing can be read too early but LDS itself, behind wait_for_loads and a barrier.  (With the builtin for it the compiler has every
@@ -419,7 +439,8 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const void* base, uint3
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(from), "s"(base) : "memory");
 }
 // (The builtin tells the compiler, too, that its own loads are there: else it would wait for them, and with them for these, at their first use.)
-__device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); asm volatile("" ::: "memory"); }
+template <uint32_t LEFT = 0>      // all but the last LEFT loads
+__device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0x0F70 | (LEFT & 15) | LEFT >> 4 << 14); asm volatile("" ::: "memory"); }
 
 template <int DT>
 __device__ __forceinline__ lh_f32x16 product(u32x4 x, u32x4 y, lh_f32x16 c) {
@@ -427,23 +448,42 @@ __device__ __forceinline__ lh_f32x16 product(u32x4 x, u32x4 y, lh_f32x16 c) {
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lh_bf16x8, x), __builtin_bit_cast(lh_bf16x8, y), c, 0, 0, 0);
 }
 
+// A lane's columns c + 4 half .. + 3 and c + 8 + 4 half .. + 3 of its row, stored 16 bytes at a time: the lower half of the wave takes c .. c + 7
+// of its rows, the upper half the rest.  All lanes call it.
+template <int DT>
+__device__ __forceinline__ void store_pair(element_t<DT>* out, uint32_t c, uint32_t half, lh_f32x4 x, lh_f32x4 y, bool on, uint32_t dim, uint32_t wide) {
+    const uint32_t x0 = pack2<DT>(x[0], x[1]), x1 = pack2<DT>(x[2], x[3]), y0 = pack2<DT>(y[0], y[1]), y1 = pack2<DT>(y[2], y[3]);
+    const auto p = __builtin_amdgcn_permlane32_swap(x0, y0, false, false), q = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
+    const u32x4 w = {p[0], q[0], p[1], q[1]};
+    c += 8 * half;
+    if (!on) return;
+    if (wide) {
+        if (c < dim) *reinterpret_cast<u32x4*>(out + c) = w;
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) if (c + j < dim) out[c + j] = (element_t<DT>)(w[j / 2] >> 16 * (j & 1));
+    }
+}
+
 // A key row's pieces are at c ^ key_place(row): rows of 16 pieces fill the banks, shorter ones do so together.
 template <uint32_t PIECES>
 __device__ __forceinline__ constexpr uint32_t key_place(uint32_t row) { return PIECES % 16 == 0 ? row & 15 : PIECES % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3; }
 
 // Many rows, 16-bit types: a workgroup per tile of 128 packed rows, kv head and split.  Each of its four waves has 32 rows, all of them
-// share the steps of KT positions, whose keys and values go from memory to LDS without registers, the next step's while this one is used.
+// share the steps of KT positions, whose keys and values go from memory to LDS without registers, ST - 1 steps ahead of their use: one step
+// where a CU has two workgroups, three where it has one and nothing else would cover the way to memory.
 //   S^T = K Q^T    32 x 32 x 16: a lane has packed row lane & 31 and half of the positions, so maximum and sum are its own registers'
 //   O^T = V^T P^T  the weights are operands where they are; V, in LDS as it is in memory, is read by the transposing ds_read_b64_tr_b16
 // In LDS the 16-byte pieces of a row change places by the row's low bits, so that neither read meets itself in one of the 64 banks: of
 // 16 neighbouring key rows the same piece is in 16 places (key_place), of four value rows the same four pieces in four.
-template <int DT, int D>
+template <int DT, int D, uint32_t ST>
 __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
     constexpr uint32_t KT = D <= 128 ? 64 : 32, SUB = KT / 32, KC = D / 16, TD = D / 32, CR = D / 8, PART = KT / 4, LOADS = PART * D / 512, kRow = D + 4;
     constexpr uint32_t VSWAP = CR % 16 == 0 ? 3 : CR % 8 == 0 ? 1 : 0;
-    constexpr bool AHEAD = D <= 128;                          // (more columns leave no registers for it)
-    extern __shared__ __align__(16) uint16_t stage[];         // [2][keys, values][KT][D]
+    constexpr bool AHEAD = D != 192;                          // (which leaves no registers for it; 256 have all of a SIMD's for one wave)
+    extern __shared__ __align__(16) uint16_t stage_memory[];
+    lds_u16* const stage = (lds_u16*)stage_memory;            // [ST][keys, values][KT][D]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, lr = lane & 31;
     const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = a.tiles - 1 - blockIdx.x / a.kv_heads / a.splits;    // long tiles first
     const Tile tile = tile_of<128>(a, t, lane);
@@ -460,8 +500,7 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
                wave_last = seen_by(a, tile, (tile.row0 + min(wave * 32 + 31, tile.count - 1)) / R);
     const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
     u32x4 qf[KC];
-#pragma unroll
-    for (uint32_t c = 0; c < KC; c++) qf[c] = query_words<DT>(a, q_at, c * 16 + half * 8, on);
+    load_query<DT>(a, q_at, half * 8, 16, on, qf);
 
     // where a lane's pieces come from, in bytes from the part's first row on
     uint32_t kfrom[LOADS], vfrom[LOADS];
@@ -486,7 +525,7 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
         }
         const uint64_t base = ((((uint64_t)pages.of(a.plan, block) * a.kv_heads + g) << a.plan.shift) + ((b * KT + wave * PART) & in_page)) * D;
         const B *K = static_cast<const B*>(a.keys) + base, *V = static_cast<const B*>(a.values) + base;
-        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)(stage + (at * 2 * KT + wave * PART) * D));
+        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(stage + (at * 2 * KT + wave * PART) * D));
 #pragma unroll
         for (uint32_t j = 0; j < LOADS; j++) load_to_lds(to + j * 1024, K, kfrom[j]);
 #pragma unroll
@@ -511,19 +550,24 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
     for (uint32_t d = 0; d < TD; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    uint32_t next_there = part.begin < part.end ? request(part.begin, 0) : 0u;
+    uint32_t theres[ST];
+    wait_for_loads();                                         // queries and table, so that the compiler waits for neither later
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < ST; i++) theres[i] = part.begin + i < part.end ? request(part.begin + i, i) : 0u;
     auto step = [&](uint32_t b, auto buffer) __attribute__((always_inline)) {
         constexpr uint32_t at = decltype(buffer)::value;      // a constant: it goes into the reads' offsets
-        const uint32_t there = next_there, p0 = b * KT;
-        wait_for_loads();
-        __syncthreads();                                      // the step is there, and nobody reads the other buffer any more
-        if (b + 1 < part.end) next_there = request(b + 1, at ^ 1);
-        const uint16_t *K = stage + at * 2 * KT * D, *V = K + KT * D;
+        const uint32_t there = theres[at], p0 = b * KT;
+        if (ST > 2 && b + ST - 2 < part.end) wait_for_loads<(ST - 2) * 2 * LOADS>();
+        else wait_for_loads();
+        __syncthreads();                                      // the step is there, and nobody reads the buffer before it any more
+        constexpr uint32_t free = (at + ST - 1) % ST;
+        if (b + ST - 1 < part.end) theres[free] = request(b + ST - 1, free);
+        const lds_u16 *K = stage + at * 2 * KT * D, *V = K + KT * D;
         if (p0 + KT > last_seen.hi || p0 < first_seen.lo || there != 15u) {      // positions that no row sees: what stands there may be anything
-            uint16_t* v = stage + (at * 2 + 1) * KT * D;
+            lds_u16* v = stage + (at * 2 + 1) * KT * D;
             for (uint32_t i = tid; i < KT * CR; i += 256) {
                 const uint32_t r = i / CR, p = p0 + r;
-                if (p >= last_seen.hi || p < first_seen.lo || !(there >> (r / PART) & 1)) *reinterpret_cast<u32x4*>(v + i * 8) = (u32x4){0, 0, 0, 0};
+                if (p >= last_seen.hi || p < first_seen.lo || !(there >> (r / PART) & 1)) *(lds_u32x4*)(v + i * 8) = (u32x4){0, 0, 0, 0};
             }
             lh_lds_barrier();
         }
@@ -533,12 +577,12 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
         u32x4 kf[2][KC], vf[2][2 * SUB];
         auto keys_of = [&](uint32_t u, u32x4 (&x)[KC]) __attribute__((always_inline)) {
 #pragma unroll
-            for (uint32_t c = 0; c < KC; c++) x[c] = *reinterpret_cast<const u32x4*>(K + kat[c % KO] + u * 32 * D + c / KO * KO * 16);
+            for (uint32_t c = 0; c < KC; c++) x[c] = *(const lds_u32x4*)(K + kat[c % KO] + u * 32 * D + c / KO * KO * 16);
         };
         auto values_of = [&](uint32_t d, u32x4 (&x)[2 * SUB]) __attribute__((always_inline)) {
 #pragma unroll
             for (uint32_t k = 0; k < 2 * SUB; k++) {
-                const uint16_t* v = V + vat[d % VO] + k * 16 * D + d / VO * VO * 32;
+                const lds_u16* v = V + vat[d % VO] + k * 16 * D + d / VO * VO * 32;
                 const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)v));
                 const uint2 z = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D)));
                 x[k] = (u32x4){y.x, y.y, z.x, z.y};
@@ -609,13 +653,20 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
             if (d + 1 == TD) __builtin_amdgcn_s_setprio(0);
         }
     };
-    for (uint32_t b = part.begin; b < part.end; b += 2) {
+    for (uint32_t b = part.begin; b < part.end; b += ST) {
         step(b, std::integral_constant<uint32_t, 0>());
         if (b + 1 < part.end) step(b + 1, std::integral_constant<uint32_t, 1>());
+        if constexpr (ST == 4) {
+            if (b + 2 < part.end) step(b + 2, std::integral_constant<uint32_t, 2>());
+            if (b + 3 < part.end) step(b + 3, std::integral_constant<uint32_t, 3>());
+        }
     }
     if (!busy) return;
     const bool alone = part.used == 1;
-    float* rec = alone ? nullptr : a.partial + (((size_t)(t * a.kv_heads + g) * a.splits + z) * 128 + wave * 32) * kRow;
+    // a record is in the order in which the waves have it: [wave][16-byte piece][lane], and maximum and sum of the 128 rows
+    float* rec = alone ? nullptr : a.partial + ((size_t)(t * a.kv_heads + g) * a.splits + z) * 128 * kRow;
+    float2* stats = reinterpret_cast<float2*>(rec + 128 * D) + wave * 32;
+    rec += wave * 32 * D;
     bool odd = false;
 #pragma unroll
     for (uint32_t d = 0; d < TD; d++)
@@ -629,27 +680,25 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
             slow_row<DT, D>(a, tile.sequence, (uint64_t)(tile.first + rw) * a.q_ld + (uint64_t)hd * a.dim, g, max(part.begin * KT, sn.lo), min(part.end * KT, sn.hi), lane, sm, sl, sums);
             const float ref = alone && a.sink ? fmaxf(sm, a.sink[hd] * kLog2e) : sm, zero = ref == -INFINITY ? 0.0f : ref, f = __builtin_amdgcn_exp2f(sm - zero);
             const float total = sl * f + (alone && a.sink ? __builtin_amdgcn_exp2f(a.sink[hd] * kLog2e - zero) : 0.0f), scale = alone ? (sl == 0.0f ? 0.0f : f / total) : 1.0f;
-            if (rec && lane == 0) { rec[r * kRow + D] = sm == -INFINITY ? 0.0f : sm; rec[r * kRow + D + 1] = sl; }
+            if (!alone && lane == 0) stats[r] = make_float2(sm == -INFINITY ? 0.0f : sm, sl);
 #pragma unroll
             for (int c = 0; c < (D + 63) / 64; c++) {
                 const uint32_t d = lane + 64 * c;
-                if (rec) { if (d < D) rec[r * kRow + d] = sums[c]; }
+                if (!alone) { if (d < D) rec[(d / 8 * 64 + d / 4 % 2 * 32 + r) * 4 + d % 4] = sums[c]; }
                 else if (d < a.dim) static_cast<B*>(a.out)[(uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim + d] = element_bits<DT>(sums[c] * scale);
             }
         }
         return;
     }
     l = lh_sum32_f(l);
-    if (!on) return;
     // a lane has columns 32 d + 8 i + 4 half .. + 3 of its row
-    if (rec) {
-        rec += lr * kRow;
+    if (!alone) {
 #pragma unroll
         for (uint32_t d = 0; d < TD; d++)
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++)
-                *reinterpret_cast<lh_f32x4*>(rec + 32 * d + 8 * i + 4 * half) = (lh_f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-        if (half == 0) { rec[D] = m == -INFINITY ? 0.0f : m; rec[D + 1] = l; }
+                *reinterpret_cast<lh_f32x4*>(rec + ((4 * d + i) * 64 + lane) * 4) = (lh_f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (half == 0) stats[lr] = make_float2(m == -INFINITY ? 0.0f : m, l);
         return;
     }
     const float sink = a.sink ? a.sink[head] * kLog2e : -INFINITY, ref = fmaxf(m, sink), zero = ref == -INFINITY ? 0.0f : ref, f = __builtin_amdgcn_exp2f(m - zero);
@@ -658,24 +707,97 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
 #pragma unroll
     for (uint32_t d = 0; d < TD; d++)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            const uint32_t c = 32 * d + 8 * i + 4 * half;
-            const uint2 x = make_uint2(pack2<DT>(o[d][4 * i] * inv, o[d][4 * i + 1] * inv), pack2<DT>(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv));
-            if (a.out_wide) {
-                if (c < a.dim) *reinterpret_cast<uint2*>(out + c) = x;
-            } else {
+        for (uint32_t i = 0; i < 4; i += 2) {
+            lh_f32x4 x, y;
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++) if (c + j < a.dim) out[c + j] = (B)((j < 2 ? x.x : x.y) >> 16 * (j & 1));
-            }
+            for (int j = 0; j < 4; j++) { x[j] = o[d][4 * i + j] * inv; y[j] = o[d][4 * i + 4 + j] * inv; }
+            store_pair<DT>(out, 32 * d + 8 * i, half, x, y, on, a.dim, a.out_wide);
         }
 }
-// Joins the splits of a tile's rows: D / 4 lanes take a split's sums, four columns each, eight splits on their way at a time, and keep a
+
+// The splits of a tile of 128 rows: a lane has two 16-byte pieces of a record, four splits on their way at a time.  MANY (more than four
+// splits): a workgroup's four waves take the splits of the same pieces in turn and meet in LDS.
+template <int DT, int D, bool MANY>
+__global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs a) {
+    typedef element_t<DT> B;
+    constexpr uint32_t kRow = D + 4, KT = D <= 128 ? 64 : 32, PAIRS = D / 16, WGS = MANY ? 4 * PAIRS : PAIRS, BATCH = 4;
+    __shared__ lh_f32x4 sums[MANY ? 4 : 1][2][64];
+    __shared__ float2 totals[MANY ? 4 : 1][64];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, half = lane >> 5, me = tid >> 6;
+    const uint32_t g = blockIdx.x / WGS % a.kv_heads, t = blockIdx.x / WGS / a.kv_heads, unit = MANY ? blockIdx.x % WGS : blockIdx.x % WGS * 4 + me;
+    const Tile tile = tile_of<128>(a, t, lane);
+    const uint32_t wave = unit / PAIRS, piece = unit % PAIRS * 2;      // of the wave that wrote them
+    if (tile.sequence < 0 || wave * 32 >= tile.count) return;
+    const uint32_t R = a.heads / a.kv_heads;
+    const Part part = part_of<KT>(a, seen_by(a, tile, tile.row0 / R).lo, seen_by(a, tile, (tile.row0 + tile.count - 1) / R).hi, 0);
+    if (part.used == 1) return;
+    const bool on = wave * 32 + (lane & 31) < tile.count;
+    const uint32_t r = min(wave * 32 + (lane & 31), tile.count - 1), pk = tile.row0 + r, rw = pk / R, hd = g * R + pk - rw * R;
+    const float* rec = a.partial + (size_t)(t * a.kv_heads + g) * a.splits * 128 * kRow;
+    const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY;
+    lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f}, y = x;
+    float m = -INFINITY, l = 0.0f;
+    // sums p, q of weight .y with maximum .x join x, y
+    auto join = [&](auto& st, auto& p, auto& q, auto count) __attribute__((always_inline)) {
+        constexpr uint32_t n = decltype(count)::value;
+        float nm = m;
+#pragma unroll
+        for (uint32_t i = 0; i < n; i++) {
+            if (st[i].y == 0.0f) { st[i].x = -INFINITY; p[i] = q[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f}; }      // nothing seen there
+            nm = fmaxf(nm, st[i].x);
+        }
+        const float zero = nm == -INFINITY ? 0.0f : nm, before = __builtin_amdgcn_exp2f(m - zero);
+        m = nm;
+        l *= before;
+#pragma unroll
+        for (int j = 0; j < 4; j++) { x[j] *= before; y[j] *= before; }
+#pragma unroll
+        for (uint32_t i = 0; i < n; i++) {
+            const float f = __builtin_amdgcn_exp2f(st[i].x - zero);
+            l += f * st[i].y;
+#pragma unroll
+            for (int j = 0; j < 4; j++) { x[j] += f * p[i][j]; y[j] += f * q[i][j]; }
+        }
+    };
+    constexpr uint32_t each = MANY ? 4 : 1;
+    for (uint32_t s0 = MANY ? me : 0; s0 < part.used; s0 += each * BATCH) {
+        lh_f32x4 p[BATCH], q[BATCH];
+        float2 st[BATCH];
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; i++) {
+            const float* from = rec + (size_t)min(s0 + i * each, part.used - 1) * 128 * kRow;
+            p[i] = *reinterpret_cast<const lh_f32x4*>(from + wave * 32 * D + (piece * 64 + lane) * 4);
+            q[i] = *reinterpret_cast<const lh_f32x4*>(from + wave * 32 * D + (piece * 64 + 64 + lane) * 4);
+            st[i] = reinterpret_cast<const float2*>(from + 128 * D)[r];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; i++) if (s0 + i * each >= part.used) st[i].y = 0.0f;
+        join(st, p, q, std::integral_constant<uint32_t, BATCH>());
+    }
+    if constexpr (MANY) {
+        sums[me][0][lane] = x; sums[me][1][lane] = y; totals[me][lane] = make_float2(m, l);
+        __syncthreads();
+        if (me) return;
+        lh_f32x4 p[3], q[3];
+        float2 st[3];
+#pragma unroll
+        for (uint32_t i = 0; i < 3; i++) { p[i] = sums[i + 1][0][lane]; q[i] = sums[i + 1][1][lane]; st[i] = totals[i + 1][lane]; }
+        join(st, p, q, std::integral_constant<uint32_t, 3>());
+    }
+    const float ref = fmaxf(m, sink), zero = ref == -INFINITY ? 0.0f : ref, f = __builtin_amdgcn_exp2f(m - zero);
+    const float inv = l == 0.0f ? 0.0f : f / (l * f + __builtin_amdgcn_exp2f(sink - zero));
+#pragma unroll
+    for (int j = 0; j < 4; j++) { x[j] *= inv; y[j] *= inv; }
+    store_pair<DT>(static_cast<B*>(a.out) + (uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim, piece * 8, half, x, y, on, a.dim, a.out_wide);
+}
+
+// The splits of a tile of 16 rows: D / 4 lanes take a split's sums, four columns each, eight splits on their way at a time, and keep a
 // running maximum of what they have seen.  FEW: these lanes are all that a row has.  Else a workgroup a row, whose
 // groups of lanes take the splits in turn and meet in LDS.
-template <int DT, int D, uint32_t ROWS, uint32_t STEP, bool FEW>
+template <int DT, int D, bool FEW>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
-    constexpr uint32_t kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS, PER = FEW ? GROUPS : 1, PARTS = (ROWS + PER - 1) / PER, BATCH = 8;
+    constexpr uint32_t ROWS = 16, STEP = 32, kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS, PER = FEW ? GROUPS : 1, PARTS = (ROWS + PER - 1) / PER, BATCH = 8;
     __shared__ lh_f32x4 sums[FEW ? 1 : 256];
     __shared__ float2 totals[GROUPS];
     const uint32_t tid = threadIdx.x, lane = tid & 63, grp = tid / QUADS, c = tid % QUADS * 4;
@@ -749,16 +871,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
 
 // How a launch is cut: tiles of all sequences at most, and parts of a tile's positions.
 struct Cut { uint64_t tiles; uint32_t splits, chunk; };
-Cut cut(uint32_t tile_rows, uint32_t step, uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t window) {
+Cut cut(uint32_t tile_rows, uint32_t step, uint32_t dim, uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t window) {
     const uint32_t R = heads / kv_heads;
     Cut c;
     c.tiles = std::min<uint64_t>((uint64_t)rows * R / tile_rows + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + tile_rows - 1) / tile_rows));
     uint64_t steps = ((uint64_t)max_length + step - 1) / step;
     if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + tile_rows + 2 * step - 2) / step);
     // Few rows: as many parts as fill the chip, or more where they would be longer than 2048 positions; none shorter than 512.  Many rows: what
-    // fills the chip twice.  (More steps never make fewer parts: a workspace is enough for every window.)
+    // the chip holds at a time (256 columns: a workgroup a CU, else two).  (More steps never make fewer parts: a workspace is enough for every window.)
     const uint64_t units = c.tiles * kv_heads, most = steps * step / (tile_rows == 16 ? 512 : 256), fewest = tile_rows == 16 && units < 4096 ? (steps * step + 2047) / 2048 : 1;
-    const uint64_t fill = tile_rows == 16 ? 2048 / units : 512 / units;
+    const uint64_t fill = (tile_rows == 16 ? 2048 : dim > 192 ? 256 : 512) / units;
     c.splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(fill, fewest), most), 1), 512);
     c.chunk = (uint32_t)std::max<uint64_t>((steps + c.splits - 1) / c.splits, 1);
     return c;
@@ -768,14 +890,14 @@ size_t cut_bytes(const Cut& c, uint32_t tile_rows, uint32_t kv_heads, uint32_t d
     return c.splits == 1 ? 0 : (size_t)c.tiles * kv_heads * c.splits * tile_rows * (lh_paged_padded_dim(dim) + 4) * 4;
 }
 
-template <int DT, int D, uint32_t ROWS, uint32_t STEP>
+template <int DT, int D>
 int launch_merge(lh_context* ctx, const PagedArgs& a, const char* op) {
     constexpr uint32_t per = 256 / (D / 4);
     // up to eight splits are on their way at once; more of them, too, where the rows fill the chip without
-    if (a.splits <= 8 || (a.splits <= 32 && (uint64_t)a.tiles * a.kv_heads * ROWS >= 4096))
-        hipLaunchKernelGGL((paged_merge_kernel<DT, D, ROWS, STEP, true>), dim3(a.tiles * a.kv_heads * ((ROWS + per - 1) / per)), dim3(256), 0, ctx->stream, a);
+    if (a.splits <= 8 || (a.splits <= 32 && (uint64_t)a.tiles * a.kv_heads * 16 >= 4096))
+        hipLaunchKernelGGL((paged_merge_kernel<DT, D, true>), dim3(a.tiles * a.kv_heads * ((16 + per - 1) / per)), dim3(256), 0, ctx->stream, a);
     else
-        hipLaunchKernelGGL((paged_merge_kernel<DT, D, ROWS, STEP, false>), dim3(a.tiles * a.kv_heads * ROWS), dim3(256), 0, ctx->stream, a);
+        hipLaunchKernelGGL((paged_merge_kernel<DT, D, false>), dim3(a.tiles * a.kv_heads * 16), dim3(256), 0, ctx->stream, a);
     return lh_check_launch(op);
 }
 template <int DT, int D>
@@ -783,13 +905,18 @@ int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op,
     int r;
     if constexpr (DT != kF32) if (tiles) {
         constexpr uint32_t KT = D <= 128 ? 64 : 32;
-        const size_t lds = (size_t)4 * KT * D * 2;
-        if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_tiles_kernel<DT, D>, lds, op)) != LH_OK) return r;
-        hipLaunchKernelGGL((paged_tiles_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
+        // (256 columns fill a CU's registers with one workgroup, 192 leave none for more steps)
+        const bool one = D > 192 || (D <= 128 && (uint64_t)a.tiles * a.kv_heads * a.splits <= (uint64_t)ctx->cu_count);
+        const size_t lds = (size_t)(one ? 4 : 2) * 2 * KT * D * 2;
+        const auto tiles_kernel = one ? paged_tiles_kernel<DT, D, D == 192 ? 2 : 4> : paged_tiles_kernel<DT, D, D <= 192 ? 2 : 4>;
+        if ((r = lh_raise_dynamic_lds(ctx, (const void*)tiles_kernel, lds, op)) != LH_OK) return r;
+        hipLaunchKernelGGL(tiles_kernel, dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
         launches = 1;
         if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
         launches = 2;
-        return launch_merge<DT, D, 128, KT>(ctx, a, op);
+        if (a.splits > 4) hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, true>), dim3(a.tiles * a.kv_heads * (D / 4)), dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, false>), dim3(a.tiles * a.kv_heads * (D / 16)), dim3(256), 0, ctx->stream, a);
+        return lh_check_launch(op);
     }
     const size_t lds = (size_t)4 * 16 * (D + 4) * 4;
     const auto rows_kernel = a.stream ? paged_rows_kernel<DT, D, true> : paged_rows_kernel<DT, D, false>;
@@ -798,7 +925,7 @@ int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op,
     launches = 1;
     if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
     launches = 2;
-    return launch_merge<DT, D, 16, 32>(ctx, a, op);
+    return launch_merge<DT, D>(ctx, a, op);
 }
 template <int DT>
 int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op, uint32_t& launches) {
@@ -822,7 +949,7 @@ size_t lh_paged_attention_workspace_bytes(uint32_t rows, uint32_t sequences, uin
     for (int dtype : {LH_BF16, LH_F32}) {
         const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
         const uint32_t n = tiles ? 128 : 16;
-        most = std::max(most, cut_bytes(cut(n, tiles ? tile_step(dim) : 32, rows, sequences, max_rows, max_length, heads, kv_heads, 0), n, kv_heads, dim));
+        most = std::max(most, cut_bytes(cut(n, tiles ? tile_step(dim) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, 0), n, kv_heads, dim));
     }
     return most;
 }
@@ -853,7 +980,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     }
     const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
     const uint32_t tile_rows = tiles ? 128 : 16;
-    const Cut c = cut(tile_rows, tiles ? tile_step(dim) : 32, rows, sequences, max_rows, max_length, heads, kv_heads, window);
+    const Cut c = cut(tile_rows, tiles ? tile_step(dim) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, window);
     if (c.splits > 1) {
         LH_NEED(workspace, cut_bytes(c, tile_rows, kv_heads, dim), op, "workspace");
         LH_REQUIRE(((uintptr_t)workspace->ptr & 15) == 0, "%s: workspace has to begin at 16 bytes", op);
