@@ -28,7 +28,7 @@ struct TurnArgs {
     uint32_t turned, key, value, items;
 };
 
-constexpr uint32_t kTurnRows = 4;          // rows of a workgroup at most
+constexpr uint32_t kTurnRows = 2;          // rows of a workgroup at most (four: 16384 rows of 32 heads of 128 45.2 us, two 42.7)
 constexpr uint32_t kTurnPairs = 1024;      // pairs whose cosines and sines fit
 
 template <typename B, int V> struct ChunkOf { typedef B type __attribute__((ext_vector_type(V))); };
@@ -37,11 +37,15 @@ template <int V, typename C> __device__ __forceinline__ auto get(const C& c, int
 template <int V, typename C, typename B> __device__ __forceinline__ void set(C& c, int i, B b) { if constexpr (V == 1) c = b; else c[i] = b; }
 
 // An item is V neighbouring values (halves: those and their partners), V * size up to 16 bytes; V = 1 takes any size and alignment
-// (neighbouring pairs: the item is a pair).
-template <int DT, int V, bool HALVES, bool APPEND>
+// (neighbouring pairs: the item is a pair).  STREAM: the rows are read with the hint that nothing reads them again.
+template <int DT, int V, bool HALVES, bool APPEND, bool STREAM>
 __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a, uint32_t per) {
     typedef element_t<DT> B;
     typedef typename ChunkOf<B, V>::type C;
+    const auto load = [](const B* p) __attribute__((always_inline)) -> C {
+        if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const C*>(p));
+        else return *reinterpret_cast<const C*>(p);
+    };
     extern __shared__ float2 turns[];                         // [per][rot / 2]
     __shared__ uint32_t at[kTurnRows], page[kTurnRows], slot[kTurnRows];
     constexpr uint32_t kNone = 0xFFFFFFFFu;
@@ -76,7 +80,7 @@ __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a, uint32_t pe
     __syncthreads();
     const uint32_t pairs = HALVES ? half / V : V == 1 ? half : a.rot / V, all = count * a.items;
     for (uint32_t it = blockIdx.y * 256 + tid; it < all; it += gridDim.y * 256) {
-        const uint32_t r = (it >= a.items) + (it >= 2 * a.items) + (it >= 3 * a.items), row = row0 + r;
+        const uint32_t r = it >= a.items, row = row0 + r;
         uint32_t k = it - r * a.items;
         const B* from;
         B* to;
@@ -102,7 +106,7 @@ __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a, uint32_t pe
             const float2* t = turns + r * half;
             if constexpr (HALVES) {
                 const uint32_t d = a.first + k * V;
-                C x = *reinterpret_cast<const C*>(from + d), y = *reinterpret_cast<const C*>(from + d + half);
+                C x = load(from + d), y = load(from + d + half);
 #pragma unroll
                 for (int i = 0; i < V; i++) {
                     const float2 cs = t[k * V + i];
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a, uint32_t pe
                 to[d + 1] = element_bits<DT>(__builtin_fmaf(w, cs.x, u * cs.y));
             } else {
                 const uint32_t d = a.first + k * V;
-                C x = *reinterpret_cast<const C*>(from + d);
+                C x = load(from + d);
 #pragma unroll
                 for (int i = 0; i < V; i += 2) {
                     const float2 cs = t[(k * V + i) / 2];
@@ -136,18 +140,18 @@ __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a, uint32_t pe
             k -= pairs;
             const uint32_t d = k * V, c = d < a.first ? d : d + a.rot;
             C x = 0;
-            if (c < a.dim) x = *reinterpret_cast<const C*>(from + c);
+            if (c < a.dim) x = load(from + c);
             *reinterpret_cast<C*>(to + c) = x;
         } else {
             const uint32_t c = k * V;
             C x = 0;
-            if (c < a.dim) x = *reinterpret_cast<const C*>(from + c);
+            if (c < a.dim) x = load(from + c);
             *reinterpret_cast<C*>(to + c) = x;
         }
     }
 }
 
-template <int DT, int V, bool APPEND>
+template <int DT, int V, bool APPEND, bool STREAM = false>
 int launch_turn(lh_context* ctx, TurnArgs& a, uint32_t pairing, const char* op) {
     const bool halves = pairing == LH_ROTARY_HALVES;
     const uint32_t pairs = halves ? a.rot / 2 / V : V == 1 ? a.rot / 2 : a.rot / V;
@@ -161,9 +165,14 @@ int launch_turn(lh_context* ctx, TurnArgs& a, uint32_t pairing, const char* op) 
     while (per > 1 && ((a.rows + per - 1) / per < 2048 || per * (a.rot / 2) > kTurnPairs)) per /= 2;
     const uint32_t groups = (a.rows + per - 1) / per, split = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, items * per / 2048), 64);
     const size_t lds = (size_t)per * (a.rot / 2) * sizeof(float2);
-    if (halves) hipLaunchKernelGGL((turn_kernel<DT, V, true, APPEND>), dim3(groups, split), dim3(256), lds, ctx->stream, a, per);
-    else hipLaunchKernelGGL((turn_kernel<DT, V, false, APPEND>), dim3(groups, split), dim3(256), lds, ctx->stream, a, per);
+    if (halves) hipLaunchKernelGGL((turn_kernel<DT, V, true, APPEND, STREAM>), dim3(groups, split), dim3(256), lds, ctx->stream, a, per);
+    else hipLaunchKernelGGL((turn_kernel<DT, V, false, APPEND, STREAM>), dim3(groups, split), dim3(256), lds, ctx->stream, a, per);
     return lh_check_launch(op);
+}
+
+template <int DT, int V, bool APPEND>
+int launch_wide(lh_context* ctx, TurnArgs& a, uint32_t pairing, bool stream, const char* op) {
+    return stream ? launch_turn<DT, V, APPEND, true>(ctx, a, pairing, op) : launch_turn<DT, V, APPEND>(ctx, a, pairing, op);
 }
 
 // The widest items that every row, head and part begins and ends with.
@@ -174,12 +183,15 @@ int launch_turn(lh_context* ctx, TurnArgs& a, int dtype, uint32_t pairing, const
     uint64_t values = a.first | a.dim | (pairing == LH_ROTARY_HALVES ? a.rot / 2 : a.rot) | a.k_ld | a.v_ld | (a.heads ? a.in_ld | a.out_ld : 0);
     bytes |= values * size;
     const uint32_t wide = (bytes & 15) == 0 ? 16 / size : (bytes & (2 * size - 1)) == 0 ? 2 : 1;
-    if (dtype == LH_F32) return wide == 4 ? launch_turn<kF32, 4, APPEND>(ctx, a, pairing, op) : wide == 2 ? launch_turn<kF32, 2, APPEND>(ctx, a, pairing, op)
-                                                                                                         : launch_turn<kF32, 1, APPEND>(ctx, a, pairing, op);
-    if (dtype == LH_F16) return wide == 8 ? launch_turn<kF16, 8, APPEND>(ctx, a, pairing, op) : wide == 2 ? launch_turn<kF16, 2, APPEND>(ctx, a, pairing, op)
-                                                                                                         : launch_turn<kF16, 1, APPEND>(ctx, a, pairing, op);
-    return wide == 8 ? launch_turn<kBf16, 8, APPEND>(ctx, a, pairing, op) : wide == 2 ? launch_turn<kBf16, 2, APPEND>(ctx, a, pairing, op)
-                                                                                      : launch_turn<kBf16, 1, APPEND>(ctx, a, pairing, op);
+    // More than stays near the chip: 16384 rows of 32 + 2 x 8 heads of 128 80 -> 64 us, their query heads 45 -> 43; 4500 rows of 16 + 2 x 4 heads, which a
+    // program's last launch has left there, 14.5 -> 19.
+    const bool stream = (uint64_t)a.rows * (a.heads + 2ull * a.kv_heads) * a.dim * size * 2 > (256ull << 20);
+    if (dtype == LH_F32) return wide == 4 ? launch_wide<kF32, 4, APPEND>(ctx, a, pairing, stream, op) : wide == 2 ? launch_turn<kF32, 2, APPEND>(ctx, a, pairing, op)
+                                                                                                                 : launch_turn<kF32, 1, APPEND>(ctx, a, pairing, op);
+    if (dtype == LH_F16) return wide == 8 ? launch_wide<kF16, 8, APPEND>(ctx, a, pairing, stream, op) : wide == 2 ? launch_turn<kF16, 2, APPEND>(ctx, a, pairing, op)
+                                                                                                                 : launch_turn<kF16, 1, APPEND>(ctx, a, pairing, op);
+    return wide == 8 ? launch_wide<kBf16, 8, APPEND>(ctx, a, pairing, stream, op) : wide == 2 ? launch_turn<kBf16, 2, APPEND>(ctx, a, pairing, op)
+                                                                                              : launch_turn<kBf16, 1, APPEND>(ctx, a, pairing, op);
 }
 
 int check_rotation(const char* op, const lh_buffer* frequencies, uint32_t dim, uint32_t rot, uint32_t first, uint32_t pairing) {
