@@ -131,8 +131,11 @@ __device__ __forceinline__ lh_f32x4 product(u32x4 x, u32x4 y, lh_f32x4 c) {
 }
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (DT == kF16) return (uint32_t)lh_f2h(a) | (uint32_t)lh_f2h(b) << 16;
-    else return lh_pack_bf(a, b);
+    if constexpr (DT == kF16) {                               // (two roundings put together are three instructions)
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+    } else return lh_pack_bf(a, b);
 }
 template <int DT>
 __device__ __forceinline__ float low(uint32_t x) { return element_value<DT>((element_t<DT>)(x & 0xFFFFu)); }
