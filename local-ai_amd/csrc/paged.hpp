@@ -75,6 +75,9 @@ inline int paged_need_rows(const char* op, const lh_buffer* b, const char* name,
     LH_REQUIRE(((uintptr_t)b->ptr & (size - 1)) == 0, "%s: %s has to begin at a value", op, name);
     return LH_OK;
 }
+inline bool paged_apart(const lh_buffer* a, size_t abytes, const lh_buffer* b, size_t bbytes) {
+    return (uintptr_t)a->ptr + abytes <= (uintptr_t)b->ptr || (uintptr_t)b->ptr + bbytes <= (uintptr_t)a->ptr;
+}
 // Whether two sets of such rows share memory.  Rows at one distance may lie side by side.
 inline bool paged_rows_meet(const lh_buffer* a, uint64_t awidth, uint32_t ald, const lh_buffer* b, uint64_t bwidth, uint32_t bld, uint32_t rows, size_t size) {
     if (rows == 0 || awidth == 0 || bwidth == 0) return false;

@@ -975,6 +975,9 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     if ((r = paged_need_rows(op, q, "q", rows, width, q_ld, size)) != LH_OK) return r;
     if ((r = paged_need_rows(op, output, "output", rows, width, output_ld, size)) != LH_OK) return r;
     LH_REQUIRE(!paged_rows_meet(q, width, q_ld, output, width, output_ld, rows, size), "%s: q and output overlap", op);
+    const size_t pool = (size_t)pages * kv_heads * page * lh_paged_padded_dim(dim) * size, out_bytes = ((size_t)(rows - 1) * output_ld + width) * size;
+    for (const lh_buffer* p : {keys, values})
+        LH_REQUIRE(paged_apart(p, pool, output, out_bytes), "%s: output lies inside the pages", op);
     PagedArgs a{};
     if (sink) {
         LH_NEED(sink, (size_t)heads * 4, op, "sink");
@@ -985,7 +988,10 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     const uint32_t tile_rows = tiles ? 128 : 16;
     const Cut c = cut(tile_rows, tiles ? tile_step(dim) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, window);
     if (c.splits > 1) {
-        LH_NEED(workspace, cut_bytes(c, tile_rows, kv_heads, dim), op, "workspace");
+        const size_t bytes = cut_bytes(c, tile_rows, kv_heads, dim);
+        LH_NEED(workspace, bytes, op, "workspace");
+        LH_REQUIRE(paged_apart(workspace, bytes, output, out_bytes) && paged_apart(workspace, bytes, keys, pool) && paged_apart(workspace, bytes, values, pool) &&
+                       paged_apart(workspace, bytes, q, ((size_t)(rows - 1) * q_ld + width) * size), "%s: workspace overlaps what the call reads or writes", op);
         LH_REQUIRE(((uintptr_t)workspace->ptr & 15) == 0, "%s: workspace has to begin at 16 bytes", op);
         a.partial = (float*)workspace->ptr;
     }

@@ -289,15 +289,10 @@ int lh_paged_append_into(lh_batch* batch, const lh_buffer* k, const lh_buffer* v
                    "%s: q_output lies over k or v", op);
     }
     const size_t pool = (size_t)pages * kv_heads * page * lh_paged_padded_dim(dim) * size;
-    const auto apart = [&](const lh_buffer* b, size_t bytes, const lh_buffer* p) {
-        return (uintptr_t)b->ptr + bytes <= (uintptr_t)p->ptr || (uintptr_t)p->ptr + pool <= (uintptr_t)b->ptr;
-    };
-    for (const lh_buffer* p : {(const lh_buffer*)keys, (const lh_buffer*)values}) {
-        bool ok = apart(k, ((size_t)(rows - 1) * k_ld + kvw) * size, p) && apart(v, ((size_t)(rows - 1) * v_ld + kvw) * size, p);
-        if (q) ok = ok && apart(q, ((size_t)(rows - 1) * q_ld + qw) * size, p) && apart(q_output, ((size_t)(rows - 1) * q_output_ld + qw) * size, p);
-        LH_REQUIRE(ok, "%s: the rows lie inside the pages", op);
-    }
-    LH_REQUIRE(apart(keys, pool, values), "%s: keys and values have pages of their own", op);
+    const auto apart = [&](const lh_buffer* b, uint64_t width, uint32_t ld, const lh_buffer* p) { return paged_apart(b, ((size_t)(rows - 1) * ld + width) * size, p, pool); };
+    for (const lh_buffer* p : {(const lh_buffer*)keys, (const lh_buffer*)values})
+        LH_REQUIRE(apart(k, kvw, k_ld, p) && apart(v, kvw, v_ld, p) && (!q || (apart(q, qw, q_ld, p) && apart(q_output, qw, q_output_ld, p))), "%s: the rows lie inside the pages", op);
+    LH_REQUIRE(paged_apart(keys, pool, values, pool), "%s: keys and values have pages of their own", op);
     TurnArgs a{};
     if (q) { a.in = q->ptr; a.out = q_output->ptr; a.in_ld = q_ld; a.out_ld = q_output_ld; }
     a.heads = heads; a.dim = dim; a.rot = rot; a.first = rot ? first : 0; a.rows = rows;

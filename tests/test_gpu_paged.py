@@ -178,6 +178,13 @@ def test_append_drops_what_has_no_page(dev, dtype):
     check_append(step, dtype, 64, 0, True, *run_append(dev, step, dtype, 2, 1, 64, 64, 0, True, 6))
 
 
+def test_append_of_a_length_beyond_every_table(dev):
+    step = Step([(3, 40), (4, 20)], 16, seed=4)
+    step.sequences[0] = (3, 0xFFFFFFFF)
+    step.lengths[0] = 0xFFFFFFFF
+    check_append(step, "bf16", 64, 0, True, *run_append(dev, step, "bf16", 2, 1, 64, 64, 0, True, 6))
+
+
 def test_append_of_a_sequence_that_ends_behind_the_rows_leaves_everything(dev):
     step = Step([(4, 10), (6, 10)], 16, seed=5)
     before, after = run_append(dev, step, "bf16", 2, 1, 64, 64, 0, True, 7, rows=9)     # row 9 is not there: the second sequence has none
@@ -243,6 +250,46 @@ def test_attention(dev, dtype, case):
     run_attention(dev, Step(seqs, page, seed=case), dtype, heads, G, dim, window, sink, seed=case, spread=1.0 + 2.0 * (case % 2))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,G,dim,window", [(32, 8, 64, 0), (32, 8, 128, 0), (16, 8, 32, 300), (32, 8, 192, 0), (16, 8, 250, 0)])
+def test_attention_of_more_tiles_than_the_chip_has_units(dev, dtype, heads, G, dim, window):
+    run_attention(dev, Step([(640, 820), (90, 90), (1, 300), (37, 512)], 16, seed=dim), dtype, heads, G, dim, window, seed=dim)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [32, 64, 128, 192, 256])
+@pytest.mark.parametrize("rows,window,sink", [(1, 0, True), (20, 0, False), (20, 2900, True)])
+def test_attention_over_long_caches_in_many_parts(dev, dtype, dim, rows, window, sink):
+    run_attention(dev, Step([(rows, 6000), (1, 40), (rows, 2000)], 64, seed=dim), dtype, 8, 2, dim, window, sink, seed=dim, spread=3.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_of_many_tokens_over_long_caches(dev, dtype):
+    """More than eight parts of rows that fill the chip; the sequences hold the same pages, to different lengths."""
+    lengths = [17000 - 13 * i for i in range(40)]
+    step = Step([(1, n) for n in lengths], 128, seed=1)
+    own = step.table[0].copy()
+    step.table[:] = own
+    rank = {int(p): i for i, p in enumerate(sorted(int(p) for p in own if p != NO_PAGE))}
+    step.pages = len(rank)
+    step.table = np.vectorize(lambda p: rank.get(int(p), NO_PAGE))(step.table).astype(np.uint32)
+    run_attention(dev, step, dtype, 8, 8, 32, seed=4)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_of_lengths_beyond_everything(dev, dtype, rows):
+    """A length that no table reaches: the row sees what the table has."""
+    step = Step([(rows, 200), (1, 50)], 16, seed=3, table_extra=0)
+    step.sequences[0] = (rows, 0xFFFFFFFF)
+    step.lengths[0], step.max_length = 0xFFFFFFFF, 1 << 20
+    run_attention(dev, step, dtype, 4, 2, 64, seed=2)
+    step = Step([(rows, 200), (1, 50)], 16, seed=3)
+    step.sequences[0] = (rows, 0xFFFFFFFF)
+    step.lengths[0], step.max_length = 0xFFFFFFFF, 170
+    run_attention(dev, step, dtype, 4, 2, 64, window=1 << 31, seed=2)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim,lead,pad", [(64, 4, 0), (80, 0, 3), (50, 2, 1), (128, 0, 8)])
 def test_attention_of_rows_at_odd_places(dev, dtype, dim, lead, pad):
@@ -259,21 +306,21 @@ def test_attention_scales(dev, dtype, rows, scale):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 60])
-@pytest.mark.parametrize("window", [0, 100])
-def test_attention_does_not_see_what_is_masked(dev, dtype, rows, window):
+@pytest.mark.parametrize("window,length", [(0, 333), (100, 333), (0, 3300), (2000, 3300)])
+def test_attention_does_not_see_what_is_masked(dev, dtype, rows, window, length):
     """NaN and infinities in slots behind a sequence's end, in front of its window, on pages of nobody -- and at positions that some rows see
     and others do not, where only the rows that see them may have them."""
-    step = Step([(rows, 333), (rows, 64), (1, 30)], 32, seed=6)
+    step = Step([(rows, length), (rows, 64), (1, 30)], 32, seed=6)
     G, dim = 2, 128
     shape = (step.pages, G, step.page, 128)
     keys, values = normal(1, *shape, dtype=dtype), normal(2, *shape, dtype=dtype)
     mine = torch.zeros(shape[0], shape[2], dtype=torch.bool)
-    for s, (n, length) in enumerate(step.sequences):
-        for p in range(max(0, length - n + 1 - window) if window else 0, length):
+    for s, (n, end) in enumerate(step.sequences):
+        for p in range(max(0, end - n + 1 - window) if window else 0, end):
             mine[int(step.table[s, p // 32]), p % 32] = True
     for x, bad in ((keys, math.nan), (values, math.nan)):
         x.permute(0, 2, 1, 3)[~mine] = bad
-    last = int(step.table[0, 332 // 32]), 332 % 32                 # the first sequence's last position: its last row alone sees it
+    last = int(step.table[0, (length - 1) // 32]), (length - 1) % 32                 # the first sequence's last position: its last row alone sees it
     values[last[0], 0, last[1], 3] = math.inf
     values[last[0], 1, last[1], 5] = math.nan
     keys[int(step.table[1, 63 // 32]), 0, 63 % 32] = math.nan

@@ -214,5 +214,7 @@ def test_attention_refusals(pkg):
                     dict(lengths=None), dict(rows=7), dict(sequences=4), dict(sequences=0), dict(max_rows=0), dict(max_rows=7), dict(heads=0), dict(heads=7), dict(kv_heads=3), dict(kv_heads=0),
                     dict(dim=0), dict(dim=101), dict(dim=300), dict(pages=2001), dict(page=17), dict(table_ld=1001), dict(q_ld=700), dict(output_ld=799), dict(output_ld=801),
                     dict(scale=math.nan), dict(scale=math.inf), dict(sink=buf(8 * GB, 31)), dict(sink=buf(8 * GB + 2, 32)), dict(workspace=None), dict(workspace=buf(9 * GB, need - 1)),
-                    dict(workspace=buf(9 * GB + 4, need)), dict(output=buf(GB, 6 * 800 * 2)), dict(output=buf(GB + 6 * 1600 - 2, 6 * 800 * 2)), dict(keys=buf(3 * GB + 2, pool))):
+                    dict(workspace=buf(9 * GB + 4, need)), dict(output=buf(GB, 6 * 800 * 2)), dict(output=buf(GB + 6 * 1600 - 2, 6 * 800 * 2)), dict(keys=buf(3 * GB + 2, pool)),
+                    dict(output=buf(4 * GB + pool - 2, 6 * 800 * 2)), dict(workspace=buf(2 * GB + 6 * 1600 - 16, need)), dict(workspace=buf(GB - need + 16, need)),
+                    dict(workspace=buf(3 * GB + 16, need))):
         c.refused(**changed)
