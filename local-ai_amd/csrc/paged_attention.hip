@@ -16,6 +16,9 @@ typedef _Float16 lh_f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Positions of a step of the kernel for many rows, by the padded columns of a head.
+__host__ __device__ constexpr uint32_t tile_step(uint32_t columns) { return columns <= 128 ? 64 : 32; }
+
 struct PagedArgs {
     const void *q, *keys, *values;
     void* out;
@@ -442,8 +445,7 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const void* base, uint3
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(from), "s"(base) : "memory");
 }
 // (The builtin tells the compiler, too, that its own loads are there: else it would wait for them, and with them for these, at their first use.)
-template <uint32_t LEFT = 0>      // all but the last LEFT loads
-__device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0x0F70 | (LEFT & 15) | LEFT >> 4 << 14); asm volatile("" ::: "memory"); }
+__device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); asm volatile("" ::: "memory"); }
 
 template <int DT>
 __device__ __forceinline__ lh_f32x16 product(u32x4 x, u32x4 y, lh_f32x16 c) {
@@ -473,20 +475,19 @@ template <uint32_t PIECES>
 __device__ __forceinline__ constexpr uint32_t key_place(uint32_t row) { return PIECES % 16 == 0 ? row & 15 : PIECES % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3; }
 
 // Many rows, 16-bit types: a workgroup per tile of 128 packed rows, kv head and split.  Each of its four waves has 32 rows, all of them
-// share the steps of KT positions, whose keys and values go from memory to LDS without registers, ST - 1 steps ahead of their use: one step
-// where a CU has two workgroups, three where it has one and nothing else would cover the way to memory.
+// share the steps of KT positions, whose keys and values go from memory to LDS without registers, the next step's while this one is used.
 //   S^T = K Q^T    32 x 32 x 16: a lane has packed row lane & 31 and half of the positions, so maximum and sum are its own registers'
 //   O^T = V^T P^T  the weights are operands where they are; V, in LDS as it is in memory, is read by the transposing ds_read_b64_tr_b16
 // In LDS the 16-byte pieces of a row change places by the row's low bits, so that neither read meets itself in one of the 64 banks: of
 // 16 neighbouring key rows the same piece is in 16 places (key_place), of four value rows the same four pieces in four.
-template <int DT, int D, uint32_t ST>
+template <int DT, int D>
 __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
-    constexpr uint32_t KT = D <= 128 ? 64 : 32, SUB = KT / 32, KC = D / 16, TD = D / 32, CR = D / 8, PART = KT / 4, LOADS = PART * D / 512, kRow = D + 4;
+    constexpr uint32_t KT = tile_step(D), SUB = KT / 32, KC = D / 16, TD = D / 32, CR = D / 8, PART = KT / 4, LOADS = PART * D / 512, kRow = D + 4;
     constexpr uint32_t VSWAP = CR % 16 == 0 ? 3 : CR % 8 == 0 ? 1 : 0;
     constexpr bool AHEAD = D != 192;                          // (which leaves no registers for it; 256 have all of a SIMD's for one wave)
     extern __shared__ __align__(16) uint16_t stage_memory[];
-    lds_u16* const stage = (lds_u16*)stage_memory;            // [ST][keys, values][KT][D]
+    lds_u16* const stage = (lds_u16*)stage_memory;            // [2][keys, values][KT][D]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, lr = lane & 31;
     const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = a.tiles - 1 - blockIdx.x / a.kv_heads / a.splits;    // long tiles first
     const Tile tile = tile_of<128>(a, t, lane);
@@ -553,18 +554,14 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
     for (uint32_t d = 0; d < TD; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    uint32_t theres[ST];
     wait_for_loads();                                         // queries and table, so that the compiler waits for neither later
-#pragma unroll
-    for (uint32_t i = 0; i + 1 < ST; i++) theres[i] = part.begin + i < part.end ? request(part.begin + i, i) : 0u;
+    uint32_t next_there = part.begin < part.end ? request(part.begin, 0) : 0u;
     auto step = [&](uint32_t b, auto buffer) __attribute__((always_inline)) {
         constexpr uint32_t at = decltype(buffer)::value;      // a constant: it goes into the reads' offsets
-        const uint32_t there = theres[at], p0 = b * KT;
-        if (ST > 2 && b + ST - 2 < part.end) wait_for_loads<(ST - 2) * 2 * LOADS>();
-        else wait_for_loads();
-        __syncthreads();                                      // the step is there, and nobody reads the buffer before it any more
-        constexpr uint32_t free = (at + ST - 1) % ST;
-        if (b + ST - 1 < part.end) theres[free] = request(b + ST - 1, free);
+        const uint32_t there = next_there, p0 = b * KT;
+        wait_for_loads();
+        __syncthreads();                                      // the step is there, and nobody reads the other buffer any more
+        if (b + 1 < part.end) next_there = request(b + 1, at ^ 1);
         const lds_u16 *K = stage + at * 2 * KT * D, *V = K + KT * D;
         if (p0 + KT > last_seen.hi || p0 < first_seen.lo || there != 15u) {      // positions that no row sees: what stands there may be anything
             lds_u16* v = stage + (at * 2 + 1) * KT * D;
@@ -656,13 +653,9 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
             if (d + 1 == TD) __builtin_amdgcn_s_setprio(0);
         }
     };
-    for (uint32_t b = part.begin; b < part.end; b += ST) {
+    for (uint32_t b = part.begin; b < part.end; b += 2) {
         step(b, std::integral_constant<uint32_t, 0>());
         if (b + 1 < part.end) step(b + 1, std::integral_constant<uint32_t, 1>());
-        if constexpr (ST == 4) {
-            if (b + 2 < part.end) step(b + 2, std::integral_constant<uint32_t, 2>());
-            if (b + 3 < part.end) step(b + 3, std::integral_constant<uint32_t, 3>());
-        }
     }
     if (!busy) return;
     const bool alone = part.used == 1;
@@ -723,7 +716,7 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
 template <int DT, int D, bool MANY>
 __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
-    constexpr uint32_t kRow = D + 4, KT = D <= 128 ? 64 : 32, PAIRS = D / 16, WGS = MANY ? 4 * PAIRS : PAIRS, BATCH = 4;
+    constexpr uint32_t kRow = D + 4, KT = tile_step(D), PAIRS = D / 16, WGS = MANY ? 4 * PAIRS : PAIRS, BATCH = 4;
     __shared__ lh_f32x4 sums[MANY ? 4 : 1][2][64];
     __shared__ float2 totals[MANY ? 4 : 1][64];
     const uint32_t tid = threadIdx.x, lane = tid & 63, half = lane >> 5, me = tid >> 6;
@@ -907,13 +900,10 @@ template <int DT, int D>
 int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op, uint32_t& launches) {
     int r;
     if constexpr (DT != kF32) if (tiles) {
-        constexpr uint32_t KT = D <= 128 ? 64 : 32;
-        // (256 columns fill a CU's registers with one workgroup, 192 leave none for more steps)
-        const bool one = D > 192 || (D <= 128 && (uint64_t)a.tiles * a.kv_heads * a.splits <= (uint64_t)ctx->cu_count);
-        const size_t lds = (size_t)(one ? 4 : 2) * 2 * KT * D * 2;
-        const auto tiles_kernel = one ? paged_tiles_kernel<DT, D, D == 192 ? 2 : 4> : paged_tiles_kernel<DT, D, D <= 192 ? 2 : 4>;
-        if ((r = lh_raise_dynamic_lds(ctx, (const void*)tiles_kernel, lds, op)) != LH_OK) return r;
-        hipLaunchKernelGGL(tiles_kernel, dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
+        constexpr uint32_t KT = tile_step(D);
+        const size_t lds = (size_t)4 * KT * D * 2;
+        if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_tiles_kernel<DT, D>, lds, op)) != LH_OK) return r;
+        hipLaunchKernelGGL((paged_tiles_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
         launches = 1;
         if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
         launches = 2;
@@ -940,8 +930,6 @@ int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op,
         default: return launch_rows<DT, 256>(ctx, a, tiles, op, launches);
     }
 }
-uint32_t tile_step(uint32_t dim) { return dim <= 128 ? 64 : 32; }
-
 }  // namespace
 
 extern "C" {
@@ -952,7 +940,7 @@ size_t lh_paged_attention_workspace_bytes(uint32_t rows, uint32_t sequences, uin
     for (int dtype : {LH_BF16, LH_F32}) {
         const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
         const uint32_t n = tiles ? 128 : 16;
-        most = std::max(most, cut_bytes(cut(n, tiles ? tile_step(dim) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, 0), n, kv_heads, dim));
+        most = std::max(most, cut_bytes(cut(n, tiles ? tile_step(lh_paged_padded_dim(dim)) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, 0), n, kv_heads, dim));
     }
     return most;
 }
@@ -986,7 +974,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     }
     const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
     const uint32_t tile_rows = tiles ? 128 : 16;
-    const Cut c = cut(tile_rows, tiles ? tile_step(dim) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, window);
+    const Cut c = cut(tile_rows, tiles ? tile_step(lh_paged_padded_dim(dim)) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, window);
     if (c.splits > 1) {
         const size_t bytes = cut_bytes(c, tile_rows, kv_heads, dim);
         LH_NEED(workspace, bytes, op, "workspace");
