@@ -237,8 +237,12 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint6
 //   S^T = K Q^T    a lane has packed row lane & 15 and positions 4 (lane / 16) .. + 3 of both halves of a step
 //   O^T = V^T P^T  the weights are operands where they are; of V a lane loads D / 16 neighbouring columns of its eight positions, and
 //                  pairs of positions are put together in registers, a column per product: no LDS on the way
-// Weights of 16 bits are two terms, what the first leaves being the second.
-// The next step's keys are requested when this one's are used, its values likewise.  STREAM: with the hint that nothing is read again.
+// Weights of 16 bits are two terms, what the first leaves being the second: the products are few beside the loads, and what a result is off
+// stays that of its own rounding.
+// Memory binds it: 64 tokens over 4096 to 16384 positions of 8 kv heads of 128 (2.6 GB in pages of 16 positions, runs of 4 KB) 434 us, 6.0 TB/s,
+// where reading alone reaches 6.2 to 6.8 in runs of 8 KB; 15 % of a SIMD's time is vector and matrix work.  One token over 32768 (134 MB) 23 us.
+// The next step's keys are requested when this one's are used, its values likewise (the 64 tokens 450 -> 444 us).  STREAM: with the hint that
+// nothing is read again (472 -> 450; the token, whose pages the last launch has left near the chip, 27.2 -> 28.5: from 256 MiB on).
 template <int DT, int D, bool STREAM>
 __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3 : 2) void paged_rows_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
@@ -478,6 +482,13 @@ __device__ __forceinline__ constexpr uint32_t key_place(uint32_t row) { return P
 // share the steps of KT positions, whose keys and values go from memory to LDS without registers, the next step's while this one is used.
 //   S^T = K Q^T    32 x 32 x 16: a lane has packed row lane & 31 and half of the positions, so maximum and sum are its own registers'
 //   O^T = V^T P^T  the weights are operands where they are; V, in LDS as it is in memory, is read by the transposing ds_read_b64_tr_b16
+// A weight is rounded once to 16 bits, which is what a result is off beside its own rounding: in bf16 0.0023 of it where that alone makes 0.0017.
+// (A second term as for few rows would be half as many products again.)
+// Issue binds it: 512 rows at position 16000 of 32 heads over 8 kv heads of 128 take 136 us, 1.0 PFLOP/s, at the 2.0 GHz that the chip keeps
+// there; the matrix instructions fill 47 % of a SIMD's time and the vector ones, which add to it, another 30; no bank conflicts.  Four prompts of 2048
+// to 4096 rows of 16 heads over 4: 206 us, 0.91.  The wave's priority is raised for the products (prompts 233 -> 231), operands are a group ahead
+// (chunk 157 -> 153.5), the buffers' places are constants of a loop of two steps (156 -> 153.5).  256 columns: a wave a SIMD, 2000 rows of 8 heads
+// over one 62 us, 0.53.
 // In LDS the 16-byte pieces of a row change places by the row's low bits, so that neither read meets itself in one of the 64 banks: of
 // 16 neighbouring key rows the same piece is in 16 places (key_place), of four value rows the same four pieces in four.
 template <int DT, int D>
@@ -667,7 +678,7 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
 #pragma unroll
     for (uint32_t d = 0; d < TD; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) odd = odd || o[d][i] != o[d][i];
+        for (int i = 0; i < 16; i++) odd = odd || !(fabsf(o[d][i]) < INFINITY);      // (weights above 1 may have made the infinity)
     if (__any(on && odd)) {
         for (uint32_t r = 0; r < 32 && wave * 32 + r < tile.count; r++) {
             const uint32_t pk = tile.row0 + wave * 32 + r, rw = pk / R, hd = g * R + pk - rw * R;
@@ -711,7 +722,8 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
         }
 }
 
-// The splits of a tile of 128 rows: a lane has two 16-byte pieces of a record, four splits on their way at a time.  MANY (more than four
+// The splits of a tile of 128 rows, in the order in which the waves' registers had them, so that loads and stores are whole lines (512 rows of 32 heads in four parts:
+// 10 us from rows, 8 so, and the kernel before it 3 less): a lane has two 16-byte pieces of a record, four splits on their way at a time.  MANY (more than four
 // splits): a workgroup's four waves take the splits of the same pieces in turn and meet in LDS.
 template <int DT, int D, bool MANY>
 __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs a) {
@@ -873,14 +885,17 @@ Cut cut(uint32_t tile_rows, uint32_t step, uint32_t dim, uint32_t rows, uint32_t
     c.tiles = std::min<uint64_t>((uint64_t)rows * R / tile_rows + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + tile_rows - 1) / tile_rows));
     uint64_t steps = ((uint64_t)max_length + step - 1) / step;
     if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + tile_rows + 2 * step - 2) / step);
-    // Few rows: as many parts as fill the chip, or more where they would be longer than 2048 positions; none shorter than 512.  Many rows: what
-    // the chip holds at a time (256 columns: a workgroup a CU, else two).  (More steps never make fewer parts: a workspace is enough for every window.)
+    // Few rows: as many parts as fill the chip, or more where they would be longer than 2048 positions (64 tokens of up to 16384: 439 us; 1024 444, 512 461);
+    // none shorter than 512 (a token over 32768: 27.5 us; 384 29.3, 768 30.7).  Many rows: what the chip holds at a time (256 columns: a workgroup a CU, 2000
+    // rows 71 -> 63; else two).  (More steps never make fewer parts: a workspace is enough for every window.)
     const uint64_t units = c.tiles * kv_heads, most = steps * step / (tile_rows == 16 ? 512 : 256), fewest = tile_rows == 16 && units < 4096 ? (steps * step + 2047) / 2048 : 1;
     const uint64_t fill = (tile_rows == 16 ? 2048 : dim > 192 ? 256 : 512) / units;
     c.splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(fill, fewest), most), 1), 512);
     c.chunk = (uint32_t)std::max<uint64_t>((steps + c.splits - 1) / c.splits, 1);
     return c;
 }
+// More rows of a sequence and kv head than a tile of 16 has.  64 sequences of 2000 to 8000 positions, 8 kv heads of 128: with 4 rows of 8 heads each 256 us in tiles
+// of 128 and 431 in two tiles of 16, with one row of 4 heads 493 and 438 (at 4096 to 16384).
 bool takes_tiles(int dtype, uint32_t max_rows, uint32_t heads, uint32_t kv_heads) { return dtype != LH_F32 && (uint64_t)max_rows * (heads / kv_heads) > 16; }
 size_t cut_bytes(const Cut& c, uint32_t tile_rows, uint32_t kv_heads, uint32_t dim) {
     return c.splits == 1 ? 0 : (size_t)c.tiles * kv_heads * c.splits * tile_rows * (lh_paged_padded_dim(dim) + 4) * 4;
@@ -889,7 +904,8 @@ size_t cut_bytes(const Cut& c, uint32_t tile_rows, uint32_t kv_heads, uint32_t d
 template <int DT, int D>
 int launch_merge(lh_context* ctx, const PagedArgs& a, const char* op) {
     constexpr uint32_t per = 256 / (D / 4);
-    // up to eight splits are on their way at once; more of them, too, where the rows fill the chip without
+    // up to eight splits are on their way at once; more of them, too, where the rows fill the chip without (64 tokens of 8 kv heads in 17 parts: 27 us by
+    // workgroups, 7 so; a token in 64 parts 4.6 by workgroups)
     if (a.splits <= 8 || (a.splits <= 32 && (uint64_t)a.tiles * a.kv_heads * 16 >= 4096))
         hipLaunchKernelGGL((paged_merge_kernel<DT, D, true>), dim3(a.tiles * a.kv_heads * ((16 + per - 1) / per)), dim3(256), 0, ctx->stream, a);
     else
@@ -907,6 +923,7 @@ int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op,
         launches = 1;
         if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
         launches = 2;
+        // (17 rows of 8 heads over 4 at position 6000, 23 parts: the whole call 16.9 us without the turns, 13.9 with them)
         if (a.splits > 4) hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, true>), dim3(a.tiles * a.kv_heads * (D / 4)), dim3(256), 0, ctx->stream, a);
         else hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, false>), dim3(a.tiles * a.kv_heads * (D / 16)), dim3(256), 0, ctx->stream, a);
         return lh_check_launch(op);
