@@ -196,6 +196,9 @@ __device__ __forceinline__ void load_query(const PagedArgs& a, uint64_t q_at, ui
     }
 }
 
+// Weights are 2^kLift of themselves: f16 loses bits below 2^-14, and many small weights beside a large one would all lose the same ones.
+template <int DT> constexpr float kLift = DT == kF16 ? 6.0f : 0.0f;
+
 // One packed row over positions begin .. end - 1, by one wave and value by value: what takes the place of the matrix instructions where a
 // result is not a number.  There a position that a row does not see has the weight 0, and 0 times an infinity or NaN that stands in it
 // is NaN; here it is left out.  Every lane gets the maximum (in powers of two) and the sum; sums[c] is of column lane + 64 c.
@@ -341,7 +344,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
         const float nm = fmaxf(m, lh_column_max(mx)), base_m = nm == -INFINITY ? 0.0f : nm, alpha = __builtin_amdgcn_exp2f(m - base_m);
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(p[i] - base_m); sum += p[i]; }
+        for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(p[i] - (base_m - kLift<DT>)); sum += p[i]; }
         l = l * alpha + sum;                                  // this lane's positions; the four lanes of a row are added at the end
         m = nm;
 #pragma unroll
@@ -402,7 +405,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
                 for (int i = 0; i < DL; i++) to[i] = o[i][j];
             }
         }
-        if (gr == 0) { own[lr * kRow + D] = m; own[lr * kRow + D + 1] = l; }
+        if (gr == 0) { own[lr * kRow + D] = m - kLift<DT>; own[lr * kRow + D + 1] = l; }
     }
     __syncthreads();
     const uint32_t r = tid >> 4, c0 = (tid & 15) * 4;
@@ -629,9 +632,9 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
         float ma, mb;
         lh_pair32(mx, ma, mb);
-        const float nm = fmaxf(m, fmaxf(ma, mb) * scale2);
-        // The reference of the weights follows the maximum only where that has grown 2^8 times: until then they are at most 2^8, which all
-        // types hold as exactly as 1.
+        const float nm = fmaxf(m, fmaxf(ma, mb) * scale2 - kLift<DT>);
+        // The reference of the weights follows the maximum only where that has grown 2^8 times: until then they are at most 2^8 (f16: 2^14), which
+        // all types hold as exactly as 1.
         if (__any(nm > m + 8.0f)) {
             const float alpha = __builtin_amdgcn_exp2f(m - (nm == -INFINITY ? 0.0f : nm));
             l *= alpha;
@@ -877,6 +880,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     for (int j = 0; j < 4; j++) if (c + j < a.dim) out[c + j] = element_bits<DT>(x[j] * inv);
 }
 
+constexpr uint64_t kMaxWorkgroups = 0xFFFFFF;      // of 256 threads: a launch has fewer than 2^32 threads
+
 // How a launch is cut: tiles of all sequences at most, and parts of a tile's positions.
 struct Cut { uint64_t tiles; uint32_t splits, chunk; };
 Cut cut(uint32_t tile_rows, uint32_t step, uint32_t dim, uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t window) {
@@ -1000,7 +1005,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
         LH_REQUIRE(((uintptr_t)workspace->ptr & 15) == 0, "%s: workspace has to begin at 16 bytes", op);
         a.partial = (float*)workspace->ptr;
     }
-    LH_REQUIRE(c.tiles * kv_heads * std::max(c.splits, tile_rows) < 0x7FFFFFFFull, "%s: %u rows of %u heads", op, rows, heads);
+    LH_REQUIRE(c.tiles * kv_heads * std::max(c.splits, c.splits == 1 ? 1u : 64u) <= kMaxWorkgroups, "%s: %u rows of %u heads", op, rows, heads);
     a.q = q->ptr; a.keys = keys->ptr; a.values = values->ptr; a.out = output->ptr;
     a.plan = PagedPlan{(const uint32_t*)table->ptr, (const uint32_t*)starts->ptr, (const uint32_t*)lengths->ptr, rows, sequences, table_ld, pages, (uint32_t)__builtin_ctz(page)};
     a.q_ld = q_ld; a.out_ld = output_ld;

@@ -168,6 +168,7 @@ int launch_turn(lh_context* ctx, TurnArgs& a, uint32_t pairing, const char* op) 
     uint32_t per = kTurnRows;
     while (per > 1 && ((a.rows + per - 1) / per < 2048 || per * (a.rot / 2) > kTurnPairs)) per /= 2;
     const uint32_t groups = (a.rows + per - 1) / per, split = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, items * per / 2048), 64);
+    LH_REQUIRE((uint64_t)groups * split <= 0xFFFFFF, "%s: %u rows", op, a.rows);      // a launch has fewer than 2^32 threads
     const size_t lds = (size_t)per * (a.rot / 2) * sizeof(float2);
     if (halves) hipLaunchKernelGGL((turn_kernel<DT, V, true, APPEND, STREAM>), dim3(groups, split), dim3(256), lds, ctx->stream, a, per);
     else hipLaunchKernelGGL((turn_kernel<DT, V, false, APPEND, STREAM>), dim3(groups, split), dim3(256), lds, ctx->stream, a, per);

@@ -362,7 +362,7 @@ class PagedStep:
 
     def __init__(self, ctx, tables: PageTables, rows: int, max_rows: int, max_length: int):
         self.tables, self.sequences, self.table_ld = tables, *tables.table.shape
-        self.rows, self.max_rows, self.max_length = rows, max_rows, max_length
+        self.rows, self.max_rows, self.max_length = rows, min(max_rows, rows), max_length
         self.table = Buffer.empty(ctx, tables.table.nbytes)
         self.starts = Buffer.empty(ctx, 4 * (self.sequences + 1))
         self.lengths = Buffer.empty(ctx, 4 * self.sequences)

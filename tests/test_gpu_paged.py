@@ -277,6 +277,37 @@ def test_attention_of_many_tokens_over_long_caches(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_of_many_small_weights_beside_a_large_one(dev, dtype, rows):
+    """One position with nearly all the weight, as a sequence's first often has, and thousands with 1e-5 of it each: together they weigh as much as it does when
+    there are enough of them, and below f16's normal numbers all would be off the same way.
+
+    A weight 2^-16.6 of the largest is rounded to a step of it, also where that has 16 bits: half_step of it, which the tolerance has."""
+    length, dim, G = 20000, 64, 2
+    step = Step([(rows, length)], 128, seed=3)
+    shape = (step.pages, G, 128, 64)
+    keys, values = torch.zeros(shape, dtype=TYPES[dtype]), normal(4, *shape, dtype=dtype).abs()
+    keys[..., 0] = -1.0
+    keys[int(step.table[0, 0]), :, 0, 0] = 10.5
+    values[int(step.table[0, 0]), :, 0] = -1.0
+    pkg, K = dev.pkg, dev.K
+    q = torch.zeros(rows, 4, dim, dtype=TYPES[dtype])
+    q[..., 0] = 1.0
+    out = pkg.Buffer.empty(dev.ctx, q.numel() * q.element_size())
+    need = K.paged_attention_workspace_bytes(rows, 1, rows, length, 4, G, dim)
+    K.paged_attention_into(dev.batch(), dev.up(q), dev.up(keys), dev.up(values), out, code(pkg, dtype), dev.up(step.table), dev.up(step.starts), dev.up(step.lengths), rows, 1, rows,
+                           length, 4, G, dim, step.pages, 128, step.table.shape[1], 4 * dim, 4 * dim, 1.0, 0, None, pkg.Buffer.empty(dev.ctx, max(need, 16)))
+    want, tol = attended(step, q, keys, values, 1.0)
+    assert 0.1 < float(1 / (1 + (length - rows) * math.exp(-11.5))) < 0.9
+    close(dev.down(out, q.shape, dtype), want, half_step(dtype) * want.abs() + tol + (2.0 ** -25 if dtype == "f16" else 0))
+
+
+def test_attention_of_a_thousand_sequences(dev):
+    run_attention(dev, Step([(i % 2, 1 + i % 37) for i in range(1000)] + [(3, 40)], 16, seed=1), "bf16", 4, 2, 64, seed=3)
+    run_attention(dev, Step([(i % 3, 2 + i % 37) for i in range(300)] + [(60, 200)], 16, seed=1), "f16", 4, 2, 64, seed=3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 70])
 def test_attention_of_lengths_beyond_everything(dev, dtype, rows):
     """A length that no table reaches: the row sees what the table has."""
