@@ -85,6 +85,12 @@ _ERRORS = {c.code: c for c in (NoDevice, NoCommandQueue, BufferAllocation, Libra
 
 _lib = None
 
+# Steps of a few microseconds whose arguments ctypes converts by itself: p handles, u whole numbers, f floats, in the header's order (a turned row
+# 3.0 us of the host with an object made for each, 2.0 so).
+_PROTOTYPES = {"lh_rotary_rows_into": "pppupp" + "f" + 8 * "u",
+               "lh_paged_append_into": "pppu" + 5 * "p" + 9 * "u" + "p" + "f" + 3 * "u" + "pp" + 3 * "u",
+               "lh_paged_attention_into": 5 * "p" + "u" + 3 * "p" + 12 * "u" + "f" + "u" + "pp"}
+
 
 def lib() -> C.CDLL:
     """Load ``liblocal_hip.so`` (or, where only that has been built, its bf16-weight part); raises ``LibraryCreation``
@@ -110,6 +116,8 @@ def lib() -> C.CDLL:
         _lib.lh_selective_steps_bytes.restype = C.c_size_t
         if hasattr(_lib, "lh_paged_attention_workspace_bytes"):
             _lib.lh_paged_attention_workspace_bytes.restype = C.c_size_t
+            for name, kinds in _PROTOTYPES.items():
+                getattr(_lib, name).argtypes = [{"p": C.c_void_p, "u": C.c_uint32, "f": C.c_float}[k] for k in kinds]
     return _lib
 
 
@@ -121,6 +129,16 @@ def _check(rc: int) -> None:
 
 def _u32(v) -> C.c_uint32:
     return C.c_uint32(int(v))
+
+
+def _call(f, *args) -> None:
+    """A function of _PROTOTYPES.  Whole numbers that are no ``int`` (numpy's) become one where the call does not take them."""
+    try:
+        rc = f(*args)
+    except C.ArgumentError:
+        rc = f(*[int(a) if hasattr(a, "__index__") else a for a in args])
+    if rc:
+        _check(rc)
 
 
 class Context:
@@ -970,9 +988,8 @@ class Kernels:
 
     def rotary_rows_into(self, batch, input, output, dtype, positions, frequencies, amplitude, rows, heads, dim, rot, first, pairing,
                          input_ld, output_ld):
-        _check(self._l.lh_rotary_rows_into(batch._h, input._h, output._h, C.c_int(dtype), positions._h, frequencies._h, C.c_float(amplitude),
-                                           _u32(rows), _u32(heads), _u32(dim), _u32(rot), _u32(first), _u32(pairing), _u32(input_ld),
-                                           _u32(output_ld)))
+        _call(self._l.lh_rotary_rows_into, batch._h, input._h, output._h, dtype, positions._h, frequencies._h, amplitude, rows, heads, dim, rot,
+              first, pairing, input_ld, output_ld)
 
     def paged_padded_dim(self, dim):
         return int(self._l.lh_paged_padded_dim(_u32(dim)))
@@ -980,11 +997,9 @@ class Kernels:
     def paged_append_into(self, batch, k, v, dtype, keys, values, table, starts, lengths, rows, sequences, kv_heads, dim, pages, page,
                           table_ld, k_ld, v_ld, frequencies=None, amplitude=1.0, rot=0, first=0, pairing=ROTARY_PAIRS, q=None,
                           q_output=None, heads=0, q_ld=0, q_output_ld=0):
-        _check(self._l.lh_paged_append_into(batch._h, k._h, v._h, C.c_int(dtype), keys._h, values._h, table._h, starts._h, lengths._h,
-                                            _u32(rows), _u32(sequences), _u32(kv_heads), _u32(dim), _u32(pages), _u32(page),
-                                            _u32(table_ld), _u32(k_ld), _u32(v_ld), _opt(frequencies), C.c_float(amplitude), _u32(rot),
-                                            _u32(first), _u32(pairing), _opt(q), _opt(q_output), _u32(heads), _u32(q_ld),
-                                            _u32(q_output_ld)))
+        _call(self._l.lh_paged_append_into, batch._h, k._h, v._h, dtype, keys._h, values._h, table._h, starts._h, lengths._h, rows, sequences,
+              kv_heads, dim, pages, page, table_ld, k_ld, v_ld, _opt(frequencies), amplitude, rot, first, pairing, _opt(q), _opt(q_output), heads,
+              q_ld, q_output_ld)
 
     def paged_attention_workspace_bytes(self, rows, sequences, max_rows, max_length, heads, kv_heads, dim):
         return int(self._l.lh_paged_attention_workspace_bytes(_u32(rows), _u32(sequences), _u32(max_rows), _u32(max_length), _u32(heads),
@@ -992,10 +1007,9 @@ class Kernels:
 
     def paged_attention_into(self, batch, q, keys, values, output, dtype, table, starts, lengths, rows, sequences, max_rows, max_length,
                              heads, kv_heads, dim, pages, page, table_ld, q_ld, output_ld, scale, window=0, sink=None, workspace=None):
-        _check(self._l.lh_paged_attention_into(batch._h, q._h, keys._h, values._h, output._h, C.c_int(dtype), table._h, starts._h,
-                                               lengths._h, _u32(rows), _u32(sequences), _u32(max_rows), _u32(max_length), _u32(heads),
-                                               _u32(kv_heads), _u32(dim), _u32(pages), _u32(page), _u32(table_ld), _u32(q_ld),
-                                               _u32(output_ld), C.c_float(scale), _u32(window), _opt(sink), _opt(workspace)))
+        _call(self._l.lh_paged_attention_into, batch._h, q._h, keys._h, values._h, output._h, dtype, table._h, starts._h, lengths._h, rows,
+              sequences, max_rows, max_length, heads, kv_heads, dim, pages, page, table_ld, q_ld, output_ld, scale, window, _opt(sink),
+              _opt(workspace))
 
     def linear_attention_padded_dim(self, dim):
         return int(self._l.lh_linear_attention_padded_dim(_u32(dim)))

@@ -163,6 +163,29 @@ class Call:
         assert self.pkg.lib().lh_last_error().decode().startswith("Invalid argument: ")
 
 
+def test_prototypes_are_the_headers(pkg):
+    import os
+    import re
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "local_hip.h")).read(), flags=re.S)
+    for name, kinds in pkg._PROTOTYPES.items():
+        args, = re.findall(rf"\b{name}\(([^)]*)\)", text)
+        want = "".join("p" if "*" in a else "f" if "float" in a else "u" for a in args.split(","))
+        assert kinds == want, name
+
+
+def test_whole_numbers_of_numpy_are_taken(pkg):
+    class Handle:
+        def __init__(self, h):
+            self._h = C.cast(C.pointer(h), C.c_void_p)
+    b, x = Handle(BatchHandle(None, 0)), Handle(buf(GB, 1 << 20))
+    K = pkg.Kernels.__new__(pkg.Kernels)
+    K._l = pkg.lib()
+    for u, f in ((np.int64, np.float32), (np.uint32, float), (int, np.float64)):
+        K.rotary_rows_into(b, x, x, u(2), x, x, f(1.0), u(0), u(4), u(64), u(64), u(0), u(1), u(256), u(256))
+        with pytest.raises(pkg.InvalidArgument, match="dtype 9"):
+            K.rotary_rows_into(b, x, x, u(9), x, x, f(1.0), u(0), u(4), u(64), u(64), u(0), u(1), u(256), u(256))
+
+
 def test_rotary_refusals(pkg):
     c = Call(pkg, "lh_rotary_rows_into", batch=True, input=buf(GB, 10 * 512 * 2), output=buf(2 * GB, 10 * 512 * 2), dtype=2, positions=buf(3 * GB, 40), frequencies=buf(4 * GB, 256),
              amplitude=1.0, rows=10, heads=4, dim=128, rot=128, first=0, pairing=1, input_ld=512, output_ld=512)
