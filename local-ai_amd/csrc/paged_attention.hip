@@ -19,6 +19,20 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Positions of a step of the kernel for many rows, by the padded columns of a head.
 __host__ __device__ constexpr uint32_t tile_step(uint32_t columns) { return columns <= 128 ? 64 : 32; }
 
+// n / d for n below 2^31 by a product and a shift (a division is some 30 instructions, one waiting for the other, and a launch of a few microseconds has a
+// dozen): with s = ceil(log2 d) and m = ceil(2^(31 + s) / d), m d exceeds 2^(31 + s) by less than 2^s, which n times is less than 2^(31 + s).
+struct Divisor {
+    uint32_t d, m, shift;
+    Divisor() = default;
+    explicit Divisor(uint32_t by) : d(by) {
+        uint32_t s = 0;
+        while ((1ull << s) < by) s++;
+        shift = 31 + s;
+        m = (uint32_t)(((1ull << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (uint32_t)((uint64_t)n * m >> shift); }
+};
+
 struct PagedArgs {
     const void *q, *keys, *values;
     void* out;
@@ -30,8 +44,10 @@ struct PagedArgs {
     uint32_t tiles, splits, chunk;                                 // chunk: steps that a split takes at least
     uint32_t stream;                                               // the caches are more than stays near the chip
     uint32_t q_wide, out_wide;                                     // rows, heads and their ends at 16 bytes
+    uint32_t q_plain;                                              // nothing to be done to the queries as they are loaded
     float scale2;              // of the products, in powers of two; > 0
     uint32_t negative, nothing;                                    // the scale is below zero, or zero: in the queries
+    Divisor group, by_heads, by_cut, by_chunk;                     // query heads of a kv head; kv heads; kv heads times splits; chunk
 };
 
 // The sum over this lane and the ones before it.
@@ -54,7 +70,7 @@ struct Tile {
 // All lanes get the same; sequence -1 behind the last tile.
 template <uint32_t ROWS>
 __device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t t, uint32_t lane) {
-    const uint32_t R = a.heads / a.kv_heads;
+    const uint32_t R = a.group.d;
     Tile r{-1, 0, 0, 0, 0};
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 64) {
@@ -102,7 +118,7 @@ struct Part { uint32_t begin, end, used; };
 template <uint32_t STEP>
 __device__ __forceinline__ Part part_of(const PagedArgs& a, uint32_t lo, uint32_t hi, uint32_t z) {
     const uint32_t b0 = lo / STEP, b1 = max((hi + STEP - 1) / STEP, b0), n = b1 - b0;
-    const uint32_t used = min(max((n + a.chunk - 1) / a.chunk, 1u), a.splits), per = (n + used - 1) / used;
+    const uint32_t used = min(max(a.by_chunk.of(n + a.chunk - 1), 1u), a.splits), per = used == 1 ? n : (n + used - 1) / used;
     return Part{min(b0 + z * per, b1), min(b0 + (z + 1) * per, b1), used};
 }
 
@@ -112,12 +128,12 @@ struct Pages {
     uint32_t blocks;                // entries that the wave may need
     uint32_t held, entry;           // entries held .. held + 63
     uint64_t there;                 // which of them are pages of the pool, or not needed
-    __device__ __forceinline__ void load(const PagedPlan& p, uint32_t from, uint32_t lane) {
+    __device__ __forceinline__ void ask(const PagedPlan& p, uint32_t from, uint32_t lane) {
         held = from;
-        const uint32_t i = from + lane;
-        entry = i < min(blocks, p.table_ld) ? row[i] : 0xFFFFFFFFu;
-        there = __ballot(i >= blocks || entry < p.pages);
+        entry = from + lane < min(blocks, p.table_ld) ? row[from + lane] : 0xFFFFFFFFu;
     }
+    __device__ __forceinline__ void settle(const PagedPlan& p, uint32_t lane) { there = __ballot(held + lane >= blocks || entry < p.pages); }
+    __device__ __forceinline__ void load(const PagedPlan& p, uint32_t from, uint32_t lane) { ask(p, from, lane); settle(p, lane); }
     __device__ __forceinline__ void reach(const PagedPlan& p, uint32_t block, uint32_t lane) { if (block - held >= 64) load(p, block, lane); }
     // of a block that is held: whether it is there, and its page, or some page
     __device__ __forceinline__ bool has(uint32_t block) const { return there >> (block - held) & 1; }
@@ -166,9 +182,9 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t (&x)[N]) {
 }
 
 // A lane's N pieces of 16 bytes of the query at q_at, the first at column d, `apart` columns from one to the next; zeros behind the head's
-// end and where `on` is false (q_at is a query's all the same).  The scale's sign goes into them.  All loads are on their way together.
+// end.  The scale's sign goes into them.  All loads are on their way together.
 template <int DT, int N>
-__device__ __forceinline__ void load_query(const PagedArgs& a, uint64_t q_at, uint32_t d, uint32_t apart, bool on, u32x4 (&x)[N]) {
+__device__ __forceinline__ void load_query(const PagedArgs& a, uint64_t q_at, uint32_t d, uint32_t apart, u32x4 (&x)[N]) {
     typedef element_t<DT> B;
     constexpr uint32_t n = 16 / sizeof(B);
     const B* q = static_cast<const B*>(a.q) + q_at;
@@ -187,10 +203,11 @@ __device__ __forceinline__ void load_query(const PagedArgs& a, uint64_t q_at, ui
             for (uint32_t i = 0; i < 4; i++) x[c][i] = DT == kF32 ? (uint32_t)e[i * n / 4] : (uint32_t)e[i * n / 4] | (uint32_t)e[(i * n + n / 2) / 4] << 16;
         }
     }
+    if (a.q_plain) return;
     const uint32_t sign = !a.negative ? 0u : DT == kF32 ? 0x80000000u : 0x80008000u;
 #pragma unroll
     for (int c = 0; c < N; c++) {
-        const bool in = on && !a.nothing && (!a.q_wide || d + c * apart < a.dim);
+        const bool in = !a.nothing && (!a.q_wide || d + c * apart < a.dim);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[c][i] = in ? x[c][i] ^ sign : 0u;
     }
@@ -253,28 +270,30 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
     constexpr int DL = D / 16, kRow = D + 4, KC = WIDE ? D / 16 : D / 32, VW = WIDE ? DL : DL / 2;
     extern __shared__ __align__(16) float slab[];             // [4 waves][16][kRow]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gr = lane >> 4, lr = lane & 15;
-    const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = blockIdx.x / a.kv_heads / a.splits;
+    const uint32_t t = a.by_cut.of(blockIdx.x), tz = blockIdx.x - t * a.by_cut.d, z = a.by_heads.of(tz), g = tz - z * a.kv_heads;
     const Tile tile = tile_of<16>(a, t, lane);
     if (tile.sequence < 0) return;
-    const uint32_t R = a.heads / a.kv_heads, packed = tile.row0 + min(lr, tile.count - 1), row = packed / R, head = g * R + packed - row * R;
+    const uint32_t R = a.group.d, packed = tile.row0 + min(lr, tile.count - 1), row = a.group.of(packed), head = g * R + packed - row * R;
     const bool on = lr < tile.count;
-    const uint32_t last_row = (tile.row0 + tile.count - 1) / R, first_row = tile.row0 / R;
+    const uint32_t last_row = a.group.of(tile.row0 + tile.count - 1), first_row = a.group.of(tile.row0);
     const Seen mine = seen_by(a, tile, row), first_seen = seen_by(a, tile, first_row), last_seen = seen_by(a, tile, last_row);
     const Part part = part_of<32>(a, first_seen.lo, last_seen.hi, z);
     if (z >= part.used) return;
     const uint32_t per = (part.end - part.begin + 3) / 4, begin = min(part.begin + wave * per, part.end), end = min(begin + per, part.end);
     const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
 
+    // (the table is asked first: the queries are many small pieces, and its way begins behind theirs otherwise)
+    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, (last_seen.hi + (1u << a.plan.shift) - 1) >> a.plan.shift, 0, 0, 0};
+    if (begin < end) pages.ask(a.plan, (begin * 32) >> a.plan.shift, lane);
     u32x4 qf[KC];
-    load_query<DT>(a, q_at, gr * (WIDE ? 4 : 8), WIDE ? 16 : 32, on, qf);
+    load_query<DT>(a, q_at, gr * (WIDE ? 4 : 8), WIDE ? 16 : 32, qf);
+    pages.settle(a.plan, lane);
     const float scale2 = a.scale2;
     float m = -INFINITY, l = 0.0f;
     lh_f32x4 o[DL];
 #pragma unroll
     for (int i = 0; i < DL; i++) o[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
 
-    Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, (last_seen.hi + (1u << a.plan.shift) - 1) >> a.plan.shift, 0, 0, 0};
-    if (begin < end) pages.load(a.plan, (begin * 32) >> a.plan.shift, lane);
     const uint32_t in_page = (1u << a.plan.shift) - 1;
     // Where step b's halves stand: the page's rows for this kv head, from the half's first slot on.
     uint64_t base[2];
@@ -385,7 +404,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
     l = lh_column_sum(l);
     if (__any(on && odd)) {
         for (uint32_t r = 0; r < tile.count; r++) {
-            const uint32_t pk = tile.row0 + r, rw = pk / R;
+            const uint32_t pk = tile.row0 + r, rw = a.group.of(pk);
             const Seen sn = seen_by(a, tile, rw);
             float sm, sl, sums[(D + 63) / 64];
             slow_row<DT, D>(a, tile.sequence, (uint64_t)(tile.first + rw) * a.q_ld + (uint64_t)(g * R + pk - rw * R) * a.dim, g, max(begin * 32, sn.lo), min(end * 32, sn.hi), lane, sm, sl, sums);
@@ -413,7 +432,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
     float top = -INFINITY, total = 0.0f, f[4];
 #pragma unroll
     for (int w = 0; w < 4; w++) top = fmaxf(top, slab[(w * 16 + r) * kRow + D]);
-    const uint32_t pk = tile.row0 + r, rw = pk / R, hd = g * R + pk - rw * R;
+    const uint32_t pk = tile.row0 + r, rw = a.group.of(pk), hd = g * R + pk - rw * R;
     const bool alone = part.used == 1;
     const float sink = alone && a.sink ? a.sink[hd] * kLog2e : -INFINITY, ref = fmaxf(top, sink), zero = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
@@ -503,22 +522,22 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
     extern __shared__ __align__(16) uint16_t stage_memory[];
     lds_u16* const stage = (lds_u16*)stage_memory;            // [2][keys, values][KT][D]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, lr = lane & 31;
-    const uint32_t g = blockIdx.x % a.kv_heads, z = blockIdx.x / a.kv_heads % a.splits, t = a.tiles - 1 - blockIdx.x / a.kv_heads / a.splits;    // long tiles first
+    const uint32_t tn = a.by_cut.of(blockIdx.x), tz = blockIdx.x - tn * a.by_cut.d, z = a.by_heads.of(tz), g = tz - z * a.kv_heads, t = a.tiles - 1 - tn;    // long tiles first
     const Tile tile = tile_of<128>(a, t, lane);
     if (tile.sequence < 0) return;
-    const uint32_t R = a.heads / a.kv_heads, last_row = (tile.row0 + tile.count - 1) / R;
-    const Seen first_seen = seen_by(a, tile, tile.row0 / R), last_seen = seen_by(a, tile, last_row);
+    const uint32_t R = a.group.d, last_row = a.group.of(tile.row0 + tile.count - 1);
+    const Seen first_seen = seen_by(a, tile, a.group.of(tile.row0)), last_seen = seen_by(a, tile, last_row);
     const Part part = part_of<KT>(a, first_seen.lo, last_seen.hi, z);
     if (z >= part.used) return;
     // the wave's rows
     const bool busy = wave * 32 < tile.count;
-    const uint32_t in_tile = min(wave * 32 + lr, tile.count - 1), packed = tile.row0 + in_tile, row = packed / R, head = g * R + packed - row * R;
+    const uint32_t in_tile = min(wave * 32 + lr, tile.count - 1), packed = tile.row0 + in_tile, row = a.group.of(packed), head = g * R + packed - row * R;
     const bool on = wave * 32 + lr < tile.count;
-    const Seen mine = seen_by(a, tile, row), wave_first = seen_by(a, tile, min((tile.row0 + wave * 32) / R, last_row)),
-               wave_last = seen_by(a, tile, (tile.row0 + min(wave * 32 + 31, tile.count - 1)) / R);
+    const Seen mine = seen_by(a, tile, row), wave_first = seen_by(a, tile, min(a.group.of(tile.row0 + wave * 32), last_row)),
+               wave_last = seen_by(a, tile, a.group.of(tile.row0 + min(wave * 32 + 31, tile.count - 1)));
     const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
     u32x4 qf[KC];
-    load_query<DT>(a, q_at, half * 8, 16, on, qf);
+    load_query<DT>(a, q_at, half * 8, 16, qf);
 
     // where a lane's pieces come from, in bytes from the part's first row on
     uint32_t kfrom[LOADS], vfrom[LOADS];
@@ -684,7 +703,7 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
         for (int i = 0; i < 16; i++) odd = odd || !(fabsf(o[d][i]) < INFINITY);      // (weights above 1 may have made the infinity)
     if (__any(on && odd)) {
         for (uint32_t r = 0; r < 32 && wave * 32 + r < tile.count; r++) {
-            const uint32_t pk = tile.row0 + wave * 32 + r, rw = pk / R, hd = g * R + pk - rw * R;
+            const uint32_t pk = tile.row0 + wave * 32 + r, rw = a.group.of(pk), hd = g * R + pk - rw * R;
             const Seen sn = seen_by(a, tile, rw);
             float sm, sl, sums[(D + 63) / 64];
             slow_row<DT, D>(a, tile.sequence, (uint64_t)(tile.first + rw) * a.q_ld + (uint64_t)hd * a.dim, g, max(part.begin * KT, sn.lo), min(part.end * KT, sn.hi), lane, sm, sl, sums);
@@ -735,15 +754,15 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs 
     __shared__ lh_f32x4 sums[MANY ? 4 : 1][2][64];
     __shared__ float2 totals[MANY ? 4 : 1][64];
     const uint32_t tid = threadIdx.x, lane = tid & 63, half = lane >> 5, me = tid >> 6;
-    const uint32_t g = blockIdx.x / WGS % a.kv_heads, t = blockIdx.x / WGS / a.kv_heads, unit = MANY ? blockIdx.x % WGS : blockIdx.x % WGS * 4 + me;
+    const uint32_t tg = blockIdx.x / WGS, t = a.by_heads.of(tg), g = tg - t * a.kv_heads, unit = MANY ? blockIdx.x % WGS : blockIdx.x % WGS * 4 + me;
     const Tile tile = tile_of<128>(a, t, lane);
     const uint32_t wave = unit / PAIRS, piece = unit % PAIRS * 2;      // of the wave that wrote them
     if (tile.sequence < 0 || wave * 32 >= tile.count) return;
-    const uint32_t R = a.heads / a.kv_heads;
-    const Part part = part_of<KT>(a, seen_by(a, tile, tile.row0 / R).lo, seen_by(a, tile, (tile.row0 + tile.count - 1) / R).hi, 0);
+    const uint32_t R = a.group.d;
+    const Part part = part_of<KT>(a, seen_by(a, tile, a.group.of(tile.row0)).lo, seen_by(a, tile, a.group.of(tile.row0 + tile.count - 1)).hi, 0);
     if (part.used == 1) return;
     const bool on = wave * 32 + (lane & 31) < tile.count;
-    const uint32_t r = min(wave * 32 + (lane & 31), tile.count - 1), pk = tile.row0 + r, rw = pk / R, hd = g * R + pk - rw * R;
+    const uint32_t r = min(wave * 32 + (lane & 31), tile.count - 1), pk = tile.row0 + r, rw = a.group.of(pk), hd = g * R + pk - rw * R;
     const float* rec = a.partial + (size_t)(t * a.kv_heads + g) * a.splits * 128 * kRow;
     const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY;
     lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f}, y = x;
@@ -812,11 +831,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     __shared__ lh_f32x4 sums[FEW ? 1 : 256];
     __shared__ float2 totals[GROUPS];
     const uint32_t tid = threadIdx.x, lane = tid & 63, grp = tid / QUADS, c = tid % QUADS * 4;
-    const uint32_t g = blockIdx.x / PARTS % a.kv_heads, t = blockIdx.x / PARTS / a.kv_heads, r = blockIdx.x % PARTS * PER + (FEW ? grp : 0);
+    const uint32_t tg = blockIdx.x / PARTS, t = a.by_heads.of(tg), g = tg - t * a.kv_heads, r = blockIdx.x % PARTS * PER + (FEW ? grp : 0);
     const Tile tile = tile_of<ROWS>(a, t, lane);
     if (tile.sequence < 0 || (FEW && grp >= GROUPS) || r >= tile.count) return;
-    const uint32_t R = a.heads / a.kv_heads, pk = tile.row0 + r, rw = pk / R, hd = g * R + pk - rw * R;
-    const Part part = part_of<STEP>(a, seen_by(a, tile, tile.row0 / R).lo, seen_by(a, tile, (tile.row0 + tile.count - 1) / R).hi, 0);
+    const uint32_t R = a.group.d, pk = tile.row0 + r, rw = a.group.of(pk), hd = g * R + pk - rw * R;
+    const Part part = part_of<STEP>(a, seen_by(a, tile, a.group.of(tile.row0)).lo, seen_by(a, tile, a.group.of(tile.row0 + tile.count - 1)).hi, 0);
     if (part.used == 1) return;
     const float* rec = a.partial + ((size_t)(t * a.kv_heads + g) * a.splits * ROWS + r) * kRow;
     const size_t stride = (size_t)ROWS * kRow;
@@ -1017,6 +1036,8 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     a.scale2 = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
     a.negative = scale < 0.0f; a.nothing = scale == 0.0f;
     a.stream = (uint64_t)sequences * max_length * kv_heads * 2 * lh_paged_padded_dim(dim) * size > (256ull << 20);
+    a.q_plain = a.q_wide && scale > 0.0f && dim == lh_paged_padded_dim(dim);
+    a.group = Divisor(heads / kv_heads); a.by_heads = Divisor(kv_heads); a.by_cut = Divisor(kv_heads * c.splits); a.by_chunk = Divisor(c.chunk);
     uint32_t launches = 0;
     if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, tiles, op, launches);
     else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, tiles, op, launches);
