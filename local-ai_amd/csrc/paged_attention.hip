@@ -42,7 +42,7 @@ struct PagedArgs {
     uint64_t q_ld, out_ld;
     uint32_t max_rows, heads, kv_heads, dim, window, capacity;     // capacity: positions from there on are not seen
     uint32_t tiles, splits, chunk;                                 // chunk: steps that a split takes at least
-    uint32_t stream;                                               // the caches are more than stays near the chip
+    uint32_t stream;                                               // the caches may be more than is worth keeping near the chip
     uint32_t q_wide, out_wide;                                     // rows, heads and their ends at 16 bytes
     uint32_t q_plain;                                              // nothing to be done to the queries as they are loaded
     float scale2;              // of the products, in powers of two; > 0
@@ -261,13 +261,17 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint6
 // stays that of its own rounding.
 // Memory binds it: 64 tokens over 4096 to 16384 positions of 8 kv heads of 128 (2.6 GB in pages of 16 positions, runs of 4 KB) 434 us, 6.0 TB/s,
 // where reading alone reaches 6.2 to 6.8 in runs of 8 KB; 15 % of a SIMD's time is vector and matrix work.  One token over 32768 (134 MB) 23 us.
-// The next step's keys are requested when this one's are used, its values likewise (the 64 tokens 450 -> 444 us).  STREAM: with the hint that
-// nothing is read again (472 -> 450; the token, whose pages the last launch has left near the chip, 27.2 -> 28.5: from 256 MiB on).
-template <int DT, int D, bool STREAM>
+// The next step's keys are requested when this one's are used, its values likewise (the 64 tokens 450 -> 444 us).
+// The hint that nothing is read again, for caches that would push everything else out from near the chip: 472 -> 450, the token with its pages in memory
+// 31.9 -> 28.9 (where the last launch has left them near, 26.9 -> 27.3).  Pages that sequences share are read again, and soon: 64 tokens over the same 16384
+// positions take 535 with the hint and 301 without.  So a wave looks whether the sequence before or behind its own begins with the same page here.  Nor
+// where a lane's part of a value is not 16 bytes: two pieces then touch each line twice (16 tokens of 256 columns 45 without, 51 with it).
+template <int DT, int D>
 __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3 : 2) void paged_rows_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
     constexpr bool WIDE = DT == kF32, AHEAD = !WIDE || D <= 64;      // (wider rows of 32 bits leave no registers for it)
     constexpr int DL = D / 16, kRow = D + 4, KC = WIDE ? D / 16 : D / 32, VW = WIDE ? DL : DL / 2;
+    constexpr bool HINT = VW == 4;
     extern __shared__ __align__(16) float slab[];             // [4 waves][16][kRow]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gr = lane >> 4, lr = lane & 15;
     const uint32_t t = a.by_cut.of(blockIdx.x), tz = blockIdx.x - t * a.by_cut.d, z = a.by_heads.of(tz), g = tz - z * a.kv_heads;
@@ -284,10 +288,17 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
 
     // (the table is asked first: the queries are many small pieces, and its way begins behind theirs otherwise)
     Pages pages{a.plan.table + (size_t)tile.sequence * a.plan.table_ld, (last_seen.hi + (1u << a.plan.shift) - 1) >> a.plan.shift, 0, 0, 0};
-    if (begin < end) pages.ask(a.plan, (begin * 32) >> a.plan.shift, lane);
+    bool stream = false;
+    uint32_t beside = ~0u;
+    if (begin < end) {
+        const uint32_t block = (begin * 32) >> a.plan.shift, s = tile.sequence + (lane & 1) * 2 - 1;
+        pages.ask(a.plan, block, lane);
+        if (HINT && a.stream && lane < 2 && s < a.plan.sequences && block < a.plan.table_ld) beside = a.plan.table[(size_t)s * a.plan.table_ld + block];
+    }
     u32x4 qf[KC];
     load_query<DT>(a, q_at, gr * (WIDE ? 4 : 8), WIDE ? 16 : 32, qf);
     pages.settle(a.plan, lane);
+    if (HINT && a.stream) stream = !__ballot(lane < 2 && beside == (uint32_t)__builtin_amdgcn_readfirstlane(pages.entry));
     const float scale2 = a.scale2;
     float m = -INFINITY, l = 0.0f;
     lh_f32x4 o[DL];
@@ -309,22 +320,34 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
     };
     u32x4 kf[2][KC];
     uint32_t v[2][4][VW];
-    auto load_keys = [&]() __attribute__((always_inline)) {
+    auto keys_of = [&](auto hint) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const B* K = static_cast<const B*>(a.keys) + base[h] + lr * D + gr * (WIDE ? 4 : 8);
 #pragma unroll
-            for (int c = 0; c < KC; c++) kf[h][c] = load16<STREAM>(K + c * (WIDE ? 16 : 32));
+            for (int c = 0; c < KC; c++) kf[h][c] = load16<hint()>(K + c * (WIDE ? 16 : 32));
         }
     };
-    auto load_values = [&]() __attribute__((always_inline)) {
+    auto values_of = [&](auto hint) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const B* V = static_cast<const B*>(a.values) + base[h] + gr * 4 * D + lr * DL;
 #pragma unroll
-            for (int j = 0; j < 4; j++) load_words<STREAM>(V + j * D, v[h][j]);
+            for (int j = 0; j < 4; j++) load_words<hint()>(V + j * D, v[h][j]);
         }
     };
+    // (both ways are the same loads but for the hint, and the compiler would make one without it of them)
+    auto by_hint = [&](auto&& load) __attribute__((always_inline)) {
+        if constexpr (HINT) if (stream) {
+            asm volatile("" ::: "memory");
+            load(std::true_type{});
+            asm volatile("" ::: "memory");
+            return;
+        }
+        load(std::false_type{});
+    };
+    auto load_keys = [&]() __attribute__((always_inline)) { by_hint(keys_of); };
+    auto load_values = [&]() __attribute__((always_inline)) { by_hint(values_of); };
     if (AHEAD && begin < end) { locate(begin); load_keys(); load_values(); }
     for (uint32_t b = begin; b < end; b++) {
         if (!AHEAD) { locate(b); load_keys(); load_values(); }
@@ -953,9 +976,8 @@ int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op,
         return lh_check_launch(op);
     }
     const size_t lds = (size_t)4 * 16 * (D + 4) * 4;
-    const auto rows_kernel = a.stream ? paged_rows_kernel<DT, D, true> : paged_rows_kernel<DT, D, false>;
-    if ((r = lh_raise_dynamic_lds(ctx, (const void*)rows_kernel, lds, op)) != LH_OK) return r;
-    hipLaunchKernelGGL(rows_kernel, dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
+    if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_rows_kernel<DT, D>, lds, op)) != LH_OK) return r;
+    hipLaunchKernelGGL((paged_rows_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
     launches = 1;
     if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
     launches = 2;
@@ -1035,7 +1057,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     a.out_wide = (((uintptr_t)a.out | (uint64_t)output_ld * size | (uint64_t)dim * size) & 15) == 0;
     a.scale2 = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
     a.negative = scale < 0.0f; a.nothing = scale == 0.0f;
-    a.stream = (uint64_t)sequences * max_length * kv_heads * 2 * lh_paged_padded_dim(dim) * size > (256ull << 20);
+    a.stream = (uint64_t)sequences * max_length * kv_heads * 2 * lh_paged_padded_dim(dim) * size > (32ull << 20);
     a.q_plain = a.q_wide && scale > 0.0f && dim == lh_paged_padded_dim(dim);
     a.group = Divisor(heads / kv_heads); a.by_heads = Divisor(kv_heads); a.by_cut = Divisor(kv_heads * c.splits); a.by_chunk = Divisor(c.chunk);
     uint32_t launches = 0;

@@ -383,6 +383,19 @@ def test_attention_of_shared_pages_and_one_sequence_twice(dev):
     run_attention(dev, step, "bf16", 8, 2, 128, seed=10)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_of_sequences_with_and_without_a_common_beginning(dev, dtype, dim):
+    """Caches that may be long, whose sequences share all, some or none of their pages with the ones beside them."""
+    step = Step([(1, 3000), (1, 3000), (2, 2900), (0, 500), (1, 2600), (1, 40), (1, 0), (1, 1300)], 32, seed=dim)
+    step.table[1, :60] = step.table[0, :60]
+    step.table[2, :] = step.table[1, :]
+    step.table[3, :] = step.table[4, :]
+    step.table[4, 7] = NO_PAGE
+    run_attention(dev, step, dtype, 8, 2, dim, seed=dim, max_length=40000)
+    run_attention(dev, step, dtype, 8, 2, dim, 700, True, seed=dim + 1, max_length=40000)
+
+
 def test_attention_of_no_sequence_and_of_one_that_ends_behind_the_rows(dev):
     step = Step([(0, 10), (0, 0)], 16, seed=1)
     run_attention(dev, step, "bf16", 4, 2, 64, rows=3)
