@@ -41,13 +41,16 @@ struct PagedArgs {
     PagedPlan plan;
     uint64_t q_ld, out_ld;
     uint32_t max_rows, heads, kv_heads, dim, window, capacity;     // capacity: positions from there on are not seen
-    uint32_t tiles, splits, chunk;                                 // chunk: steps that a split takes at least
+    uint32_t most, least, fill, share, coarse, fixed;              // how tiles are cut (chunk_of): steps of a tile at most and of a part at least; workgroups wanted,
+                                                                   // and of a kv head; what the sum is shifted by; nothing to measure
+    uint32_t parts;                                                // of all tiles at most
+    uint32_t records, rows_kept;                                   // records of a kv head that the workspace takes; rows of one
     uint32_t stream;                                               // the caches may be more than is worth keeping near the chip
     uint32_t q_wide, out_wide;                                     // rows, heads and their ends at 16 bytes
     uint32_t q_plain;                                              // nothing to be done to the queries as they are loaded
     float scale2;              // of the products, in powers of two; > 0
     uint32_t negative, nothing;                                    // the scale is below zero, or zero: in the queries
-    Divisor group, by_heads, by_cut, by_chunk;                     // query heads of a kv head; kv heads; kv heads times splits; chunk
+    Divisor group, by_heads;                                       // query heads of a kv head; kv heads
 };
 
 // The sum over this lane and the ones before it.
@@ -61,44 +64,101 @@ __device__ __forceinline__ uint32_t sum_up_to(uint32_t v) {
     return v;
 }
 
-// A tile of a sequence: its rows row0 .. row0 + count - 1 of the packed ones.
+// n / d rounded down, or one less: by the reciprocal (good to 2^-22), for quotients below 2^20.
+__device__ __forceinline__ uint32_t about(uint32_t n, uint32_t d) {
+    const uint32_t q = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));
+    return q * d > n ? q - 1 : q;
+}
+__device__ __forceinline__ uint32_t whole(uint32_t n, uint32_t d) {
+    const uint32_t q = about(n, d);
+    return n - q * d >= d ? q + 1 : q;
+}
+
+// What a lane's sequence has: tiles, and steps of positions that each may take at most.
+struct Load { uint32_t first, all, length, tiles, steps; };
+template <uint32_t ROWS, uint32_t STEP>
+__device__ __forceinline__ Load load_of(const PagedArgs& a, uint32_t s) {
+    Load c{0, 0, 0, 0, 0};
+    if (s < a.plan.sequences) {
+        c.first = a.plan.starts[s];
+        c.length = a.plan.lengths[s];
+        const uint32_t end = a.plan.starts[s + 1];
+        if (end > c.first && end <= a.plan.rows) {
+            c.all = end - c.first;
+            c.tiles = (uint32_t)(((uint64_t)min(c.all, a.max_rows) * a.group.d + ROWS - 1) / ROWS);
+            c.steps = min((min(c.length, a.capacity) + STEP - 1) / STEP, a.most);
+        }
+    }
+    return c;
+}
+
+// Steps of a part: what all tiles have to do over the workgroups wanted, so that a long sequence among short ones is cut and short ones alone are not, whatever bound the
+// call gives for their lengths (64 tokens at 4000 of a call for up to 131072: parts by the bound 313 us, so 171; 256 at 1000 653 and 174).  Where there are few tiles,
+// equal ones make a whole number of parts.  It costs every workgroup two scans and a reciprocal, 0.5 us.  All kernels of a call find the same.
+//   The sum is of steps shifted by `coarse` and rounded up, which lets it fit.  The chunk is at least what all have over `share`: so the parts of all tiles are at most
+//   `share` more than there are tiles, and, a tile in parts having more than a chunk, those of such tiles at most twice `share`.
+template <uint32_t ROWS, uint32_t STEP>
+__device__ __forceinline__ uint32_t chunk_of(const PagedArgs& a, uint32_t lane, Load& c) {
+    uint32_t tiles = 0, work = 0;
+    for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 64) {
+        c = load_of<ROWS, STEP>(a, s0 + lane);
+        tiles += c.tiles;
+        work += (uint32_t)(((uint64_t)c.tiles * c.steps + (1ull << a.coarse) - 1) >> a.coarse);
+    }
+    if (a.fixed) return a.least;
+    tiles = __builtin_amdgcn_readlane(sum_up_to(tiles), 63);
+    work = __builtin_amdgcn_readlane(sum_up_to(work), 63);
+    const uint64_t units = (uint64_t)tiles * a.kv_heads;
+    // (a reciprocal's error cannot take the quotient over a whole number, nor the chunk below what it has to be)
+    const float each = units >= a.fill ? 0.0f : __builtin_truncf((float)a.fill * __builtin_amdgcn_rcpf((float)max((uint32_t)units, 1u)) * 1.00001f);
+    const float parts = units >= a.fill ? (float)a.share : max((float)tiles, 1.0f) * each;
+    const uint32_t steps = (uint32_t)((float)work * __builtin_amdgcn_rcpf(parts) * 1.00001f) + 1;
+    return max((uint32_t)min((uint64_t)steps << a.coarse, (uint64_t)a.most), a.least);
+}
+
+// A tile of a sequence: its rows row0 .. row0 + count - 1 of the packed ones; and part `split` of it.
 struct Tile {
     int sequence;
     uint32_t row0, count, first;    // first: the sequence's first row in q
     int64_t begin;                  // position of the sequence's first row
+    uint32_t split, parts, chunk;   // parts: at most
+    uint32_t record;                // records of a kv head before its own, where it has several parts
+    // The first record for kv head g; its parts' follow.
+    __device__ __forceinline__ size_t record_of(const PagedArgs& a, uint32_t g) const { return (size_t)record * a.kv_heads + (size_t)g * parts; }
 };
-// All lanes get the same; sequence -1 behind the last tile.
-template <uint32_t ROWS>
-__device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t t, uint32_t lane) {
+// Part n of all tiles, JOIN: tile n of those in parts.  All lanes get the same; sequence -1 behind the last.  A sequence's tiles of the same part follow each other, so
+// that those that read the same pages at the same time are on different XCDs (on one, where the number of parts was a multiple of two, they waited for each
+// other: 64 rows at 8000 25.1 us, 20.4 so; 1000 rows of f32 54 and 44).
+template <uint32_t ROWS, uint32_t STEP, bool JOIN>
+__device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t n, uint32_t lane) {
     const uint32_t R = a.group.d;
-    Tile r{-1, 0, 0, 0, 0};
-    uint32_t before = 0;
+    Tile r{-1, 0, 0, 0, 0, 0, 1, 0, 0};
+    Load c;
+    r.chunk = chunk_of<ROWS, STEP>(a, lane, c);
+    uint32_t before = 0, records = 0;
     for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 64) {
-        const uint32_t s = s0 + lane;
-        uint32_t first = 0, all = 0, tiles = 0, length = 0;
-        if (s < a.plan.sequences) {
-            first = a.plan.starts[s];
-            length = a.plan.lengths[s];
-            const uint32_t end = a.plan.starts[s + 1];
-            if (end > first && end <= a.plan.rows) {
-                all = end - first;
-                tiles = (uint32_t)(((uint64_t)min(all, a.max_rows) * R + ROWS - 1) / ROWS);
-            }
-        }
-        const uint32_t sum = sum_up_to(tiles);
-        const uint64_t behind = __ballot(before + sum > t);
+        if (a.plan.sequences > 64) c = load_of<ROWS, STEP>(a, s0 + lane);
+        const uint32_t parts = max(about(c.steps + r.chunk - 1, r.chunk), 1u), all = c.tiles * parts, kept = parts > 1 ? all : 0u, size = JOIN ? (parts > 1 ? c.tiles : 0u) : all;
+        const uint32_t sum = sum_up_to(size), kept_sum = sum_up_to(kept);
+        const uint64_t behind = __ballot(before + sum > n);
         if (behind) {
             const int at = __builtin_ctzll(behind);
-            const uint32_t n = __builtin_amdgcn_readlane(all, at), rows = min(n, a.max_rows) * R;
+            const uint32_t brought = __builtin_amdgcn_readlane(c.all, at), rows = min(brought, a.max_rows) * R;
             r.sequence = s0 + at;
-            r.first = __builtin_amdgcn_readlane(first, at);
-            const uint32_t in = t - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(tiles, at));
-            r.row0 = in * ROWS;
+            r.first = __builtin_amdgcn_readlane(c.first, at);
+            r.parts = __builtin_amdgcn_readlane(parts, at);
+            const uint32_t in = n - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(size, at)), tiles = __builtin_amdgcn_readlane(c.tiles, at);
+            r.split = JOIN || r.parts == 1 ? 0u : whole(in, tiles);
+            const uint32_t i = in - r.split * tiles;
+            r.record = records + (__builtin_amdgcn_readlane(kept_sum, at) - __builtin_amdgcn_readlane(kept, at)) + i * r.parts;
+            if (i >= tiles || (r.parts > 1 && r.record + r.parts > a.records)) r.sequence = -1;      // (only where starts do not ascend: the sums say nothing then)
+            r.row0 = i * ROWS;
             r.count = min(ROWS, rows - r.row0);
-            r.begin = (int64_t)(uint32_t)__builtin_amdgcn_readlane(length, at) - n;
+            r.begin = (int64_t)(uint32_t)__builtin_amdgcn_readlane(c.length, at) - brought;
             return r;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
+        records += __builtin_amdgcn_readlane(kept_sum, 63);
     }
     return r;
 }
@@ -113,12 +173,17 @@ __device__ __forceinline__ Seen seen_by(const PagedArgs& a, const Tile& t, uint3
     return s;
 }
 
-// The part of a tile's positions that split z takes, in steps of STEP; `used` splits have any.
+// The part of a tile's positions lo .. hi - 1 that split z takes, in steps of STEP; `used` splits have any.
 struct Part { uint32_t begin, end, used; };
 template <uint32_t STEP>
-__device__ __forceinline__ Part part_of(const PagedArgs& a, uint32_t lo, uint32_t hi, uint32_t z) {
+__device__ __forceinline__ Part part_of(const Tile& t, uint32_t lo, uint32_t hi, uint32_t z) {
     const uint32_t b0 = lo / STEP, b1 = max((hi + STEP - 1) / STEP, b0), n = b1 - b0;
-    const uint32_t used = min(max(a.by_chunk.of(n + a.chunk - 1), 1u), a.splits), per = used == 1 ? n : (n + used - 1) / used;
+    const uint32_t used = t.parts == 1 ? 1u : min(max(about(n + t.chunk - 1, t.chunk), 1u), t.parts);
+    uint32_t per = n;
+    if (used > 1) {
+        per = about(n + used - 1, used) + (n >> 18);
+        per += per * used < n;
+    }
     return Part{min(b0 + z * per, b1), min(b0 + (z + 1) * per, b1), used};
 }
 
@@ -274,15 +339,15 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
     constexpr bool HINT = VW == 4;
     extern __shared__ __align__(16) float slab[];             // [4 waves][16][kRow]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gr = lane >> 4, lr = lane & 15;
-    const uint32_t t = a.by_cut.of(blockIdx.x), tz = blockIdx.x - t * a.by_cut.d, z = a.by_heads.of(tz), g = tz - z * a.kv_heads;
-    const Tile tile = tile_of<16>(a, t, lane);
+    const uint32_t n = a.by_heads.of(blockIdx.x), g = blockIdx.x - n * a.kv_heads;
+    const Tile tile = tile_of<16, 32, false>(a, n, lane);
     if (tile.sequence < 0) return;
     const uint32_t R = a.group.d, packed = tile.row0 + min(lr, tile.count - 1), row = a.group.of(packed), head = g * R + packed - row * R;
     const bool on = lr < tile.count;
     const uint32_t last_row = a.group.of(tile.row0 + tile.count - 1), first_row = a.group.of(tile.row0);
     const Seen mine = seen_by(a, tile, row), first_seen = seen_by(a, tile, first_row), last_seen = seen_by(a, tile, last_row);
-    const Part part = part_of<32>(a, first_seen.lo, last_seen.hi, z);
-    if (z >= part.used) return;
+    const Part part = part_of<32>(tile, first_seen.lo, last_seen.hi, tile.split);
+    if (tile.split >= part.used) return;
     const uint32_t per = (part.end - part.begin + 3) / 4, begin = min(part.begin + wave * per, part.end), end = min(begin + per, part.end);
     const uint64_t q_at = (uint64_t)(tile.first + row) * a.q_ld + (uint64_t)head * a.dim;
 
@@ -464,7 +529,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
         total += f[w] * slab[(w * 16 + r) * kRow + D + 1];
     }
     const float all = total + __builtin_amdgcn_exp2f(sink - zero), inv = alone ? (total == 0.0f ? 0.0f : 1.0f / all) : 1.0f;
-    float* rec = alone ? nullptr : a.partial + (((size_t)(t * a.kv_heads + g) * a.splits + z) * 16 + r) * kRow;
+    float* rec = alone ? nullptr : a.partial + ((tile.record_of(a, g) + tile.split) * a.rows_kept + r) * kRow;
     if (rec && c0 == 0) { rec[D] = zero; rec[D + 1] = total; }
     B* out = static_cast<B*>(a.out) + (uint64_t)(tile.first + rw) * a.out_ld + (uint64_t)hd * a.dim;
     for (uint32_t c = c0; c < D; c += 64) {
@@ -545,13 +610,13 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
     extern __shared__ __align__(16) uint16_t stage_memory[];
     lds_u16* const stage = (lds_u16*)stage_memory;            // [2][keys, values][KT][D]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, lr = lane & 31;
-    const uint32_t tn = a.by_cut.of(blockIdx.x), tz = blockIdx.x - tn * a.by_cut.d, z = a.by_heads.of(tz), g = tz - z * a.kv_heads, t = a.tiles - 1 - tn;    // long tiles first
-    const Tile tile = tile_of<128>(a, t, lane);
+    const uint32_t n = a.by_heads.of(blockIdx.x), g = blockIdx.x - n * a.kv_heads;
+    const Tile tile = tile_of<128, KT, false>(a, a.parts - 1 - n, lane);      // a sequence's last rows, which see most, first
     if (tile.sequence < 0) return;
     const uint32_t R = a.group.d, last_row = a.group.of(tile.row0 + tile.count - 1);
     const Seen first_seen = seen_by(a, tile, a.group.of(tile.row0)), last_seen = seen_by(a, tile, last_row);
-    const Part part = part_of<KT>(a, first_seen.lo, last_seen.hi, z);
-    if (z >= part.used) return;
+    const Part part = part_of<KT>(tile, first_seen.lo, last_seen.hi, tile.split);
+    if (tile.split >= part.used) return;
     // the wave's rows
     const bool busy = wave * 32 < tile.count;
     const uint32_t in_tile = min(wave * 32 + lr, tile.count - 1), packed = tile.row0 + in_tile, row = a.group.of(packed), head = g * R + packed - row * R;
@@ -716,7 +781,7 @@ __global__ __launch_bounds__(256, D <= 192 ? 2 : 1) void paged_tiles_kernel(cons
     if (!busy) return;
     const bool alone = part.used == 1;
     // a record is in the order in which the waves have it: [wave][16-byte piece][lane], and maximum and sum of the 128 rows
-    float* rec = alone ? nullptr : a.partial + ((size_t)(t * a.kv_heads + g) * a.splits + z) * 128 * kRow;
+    float* rec = alone ? nullptr : a.partial + (tile.record_of(a, g) + tile.split) * 128 * kRow;
     float2* stats = reinterpret_cast<float2*>(rec + 128 * D) + wave * 32;
     rec += wave * 32 * D;
     bool odd = false;
@@ -778,15 +843,16 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs 
     __shared__ float2 totals[MANY ? 4 : 1][64];
     const uint32_t tid = threadIdx.x, lane = tid & 63, half = lane >> 5, me = tid >> 6;
     const uint32_t tg = blockIdx.x / WGS, t = a.by_heads.of(tg), g = tg - t * a.kv_heads, unit = MANY ? blockIdx.x % WGS : blockIdx.x % WGS * 4 + me;
-    const Tile tile = tile_of<128>(a, t, lane);
+    const Tile tile = tile_of<128, KT, true>(a, t, lane);
     const uint32_t wave = unit / PAIRS, piece = unit % PAIRS * 2;      // of the wave that wrote them
     if (tile.sequence < 0 || wave * 32 >= tile.count) return;
     const uint32_t R = a.group.d;
-    const Part part = part_of<KT>(a, seen_by(a, tile, a.group.of(tile.row0)).lo, seen_by(a, tile, a.group.of(tile.row0 + tile.count - 1)).hi, 0);
+    const Part part = part_of<KT>(tile, seen_by(a, tile, a.group.of(tile.row0)).lo, seen_by(a, tile, a.group.of(tile.row0 + tile.count - 1)).hi, 0);
     if (part.used == 1) return;
     const bool on = wave * 32 + (lane & 31) < tile.count;
     const uint32_t r = min(wave * 32 + (lane & 31), tile.count - 1), pk = tile.row0 + r, rw = a.group.of(pk), hd = g * R + pk - rw * R;
-    const float* rec = a.partial + (size_t)(t * a.kv_heads + g) * a.splits * 128 * kRow;
+    const float* rec = a.partial + tile.record_of(a, g) * 128 * kRow;
+    const size_t stride = 128 * kRow;
     const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY;
     lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f}, y = x;
     float m = -INFINITY, l = 0.0f;
@@ -818,7 +884,7 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs 
         float2 st[BATCH];
 #pragma unroll
         for (uint32_t i = 0; i < BATCH; i++) {
-            const float* from = rec + (size_t)min(s0 + i * each, part.used - 1) * 128 * kRow;
+            const float* from = rec + min(s0 + i * each, part.used - 1) * stride;
             p[i] = *reinterpret_cast<const lh_f32x4*>(from + wave * 32 * D + (piece * 64 + lane) * 4);
             q[i] = *reinterpret_cast<const lh_f32x4*>(from + wave * 32 * D + (piece * 64 + 64 + lane) * 4);
             st[i] = reinterpret_cast<const float2*>(from + 128 * D)[r];
@@ -850,18 +916,18 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs 
 template <int DT, int D, bool FEW>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     typedef element_t<DT> B;
-    constexpr uint32_t ROWS = 16, STEP = 32, kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS, PER = FEW ? GROUPS : 1, PARTS = (ROWS + PER - 1) / PER, BATCH = 8;
+    constexpr uint32_t ROWS = 16, STEP = 32, kRow = D + 4, QUADS = D / 4, GROUPS = 256 / QUADS, PER = FEW ? GROUPS : 1, BATCH = 8;
     __shared__ lh_f32x4 sums[FEW ? 1 : 256];
     __shared__ float2 totals[GROUPS];
     const uint32_t tid = threadIdx.x, lane = tid & 63, grp = tid / QUADS, c = tid % QUADS * 4;
-    const uint32_t tg = blockIdx.x / PARTS, t = a.by_heads.of(tg), g = tg - t * a.kv_heads, r = blockIdx.x % PARTS * PER + (FEW ? grp : 0);
-    const Tile tile = tile_of<ROWS>(a, t, lane);
+    const uint32_t t = a.by_heads.of(blockIdx.x), g = blockIdx.x - t * a.kv_heads, r = blockIdx.y * PER + (FEW ? grp : 0);
+    const Tile tile = tile_of<ROWS, STEP, true>(a, t, lane);
     if (tile.sequence < 0 || (FEW && grp >= GROUPS) || r >= tile.count) return;
     const uint32_t R = a.group.d, pk = tile.row0 + r, rw = a.group.of(pk), hd = g * R + pk - rw * R;
-    const Part part = part_of<STEP>(a, seen_by(a, tile, a.group.of(tile.row0)).lo, seen_by(a, tile, a.group.of(tile.row0 + tile.count - 1)).hi, 0);
+    const Part part = part_of<STEP>(tile, seen_by(a, tile, a.group.of(tile.row0)).lo, seen_by(a, tile, a.group.of(tile.row0 + tile.count - 1)).hi, 0);
     if (part.used == 1) return;
-    const float* rec = a.partial + ((size_t)(t * a.kv_heads + g) * a.splits * ROWS + r) * kRow;
-    const size_t stride = (size_t)ROWS * kRow;
+    const float* rec = a.partial + (tile.record_of(a, g) * a.rows_kept + r) * kRow;
+    const size_t stride = (size_t)a.rows_kept * kRow;
     const float sink = a.sink ? a.sink[hd] * kLog2e : -INFINITY;
     lh_f32x4 x = (lh_f32x4){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
@@ -924,73 +990,78 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
 
 constexpr uint64_t kMaxWorkgroups = 0xFFFFFF;      // of 256 threads: a launch has fewer than 2^32 threads
 
-// How a launch is cut: tiles of all sequences at most, and parts of a tile's positions.
-struct Cut { uint64_t tiles; uint32_t splits, chunk; };
+// How a launch is cut, at most: tiles of all sequences, their parts, those that leave a record, tiles that have such.
+struct Cut { uint64_t tiles, parts, records, joins; uint32_t most, least, fill, share, coarse, fixed; };
 Cut cut(uint32_t tile_rows, uint32_t step, uint32_t dim, uint32_t rows, uint32_t sequences, uint32_t max_rows, uint32_t max_length, uint32_t heads, uint32_t kv_heads, uint32_t window) {
     const uint32_t R = heads / kv_heads;
-    Cut c;
+    Cut c{};
     c.tiles = std::min<uint64_t>((uint64_t)rows * R / tile_rows + sequences, (uint64_t)sequences * (((uint64_t)max_rows * R + tile_rows - 1) / tile_rows));
     uint64_t steps = ((uint64_t)max_length + step - 1) / step;
     if (window) steps = std::min<uint64_t>(steps, ((uint64_t)window + tile_rows + 2 * step - 2) / step);
-    // Few rows: as many parts as fill the chip, or more where they would be longer than 2048 positions (64 tokens of up to 16384: 439 us; 1024 444, 512 461);
-    // none shorter than 512 (a token over 32768: 27.5 us; 384 29.3, 768 30.7).  Many rows: what the chip holds at a time (256 columns: a workgroup a CU, 2000
-    // rows 71 -> 63; else two).  (More steps never make fewer parts: a workspace is enough for every window.)
-    const uint64_t units = c.tiles * kv_heads, most = steps * step / (tile_rows == 16 ? 512 : 256), fewest = tile_rows == 16 && units < 4096 ? (steps * step + 2047) / 2048 : 1;
-    const uint64_t fill = (tile_rows == 16 ? 2048 : dim > 192 ? 256 : 512) / units;
-    c.splits = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(fill, fewest), most), 1), 512);
-    c.chunk = (uint32_t)std::max<uint64_t>((steps + c.splits - 1) / c.splits, 1);
+    c.most = (uint32_t)steps;
+    c.least = (tile_rows == 16 ? 512 : 256) / step;
+    // Few rows: 2048 workgroups of the 768 to 1280 that run at a time (64 tokens at 4096 to 16384 424 us, at 4000 171; with 2560 416 and 176, with 4096 418 and 180);
+    // parts of 512 positions at least (a token over 32768: 27.5 us; 384 29.3, 768 30.7).  Many rows: what the chip holds at a time (256 columns: a workgroup a CU,
+    // 2000 rows 71 -> 63; else two), parts of 256 (3 times 256 rows of 256 columns
+    // and 29 tokens under a window of 512 27.5 us; 320 30.4).  Where the tiles alone fill
+    // the chip and none is longer than 128 steps, none is cut: there is no second launch (four prompts of up to 4096 rows 225 -> 219 us, 256 tokens at 1000 178 -> 167).
+    c.fill = tile_rows == 16 ? 2048 : dim > 192 ? 256 : 512;
+    c.share = std::max(c.fill / kv_heads, 1u);
+    const uint64_t units = c.tiles * kv_heads;
+    if (units >= c.fill && steps <= 128) c.least = std::max(c.least, c.most);
+    while (((c.tiles * steps) >> c.coarse) + sequences > 0x7FFFFFFFull) c.coarse++;
+    // nothing to measure where not even parts at least as long would fill the chip
+    c.fixed = c.most <= c.least || (units < c.fill && steps / (c.fill / units) + 2 <= c.least);
+    const uint64_t each = std::max<uint64_t>((steps + c.least - 1) / c.least, 1);
+    c.parts = c.tiles + std::min<uint64_t>(c.tiles * (each - 1), c.share);
+    if (each > 1) {
+        c.records = std::min<uint64_t>(c.tiles * each, 2ull * c.share);
+        c.joins = std::min<uint64_t>(c.tiles, c.share);
+    }
     return c;
 }
 // More rows of a sequence and kv head than a tile of 16 has.  64 sequences of 2000 to 8000 positions, 8 kv heads of 128: with 4 rows of 8 heads each 256 us in tiles
 // of 128 and 431 in two tiles of 16, with one row of 4 heads 493 and 438 (at 4096 to 16384).
 bool takes_tiles(int dtype, uint32_t max_rows, uint32_t heads, uint32_t kv_heads) { return dtype != LH_F32 && (uint64_t)max_rows * (heads / kv_heads) > 16; }
-size_t cut_bytes(const Cut& c, uint32_t tile_rows, uint32_t kv_heads, uint32_t dim) {
-    return c.splits == 1 ? 0 : (size_t)c.tiles * kv_heads * c.splits * tile_rows * (lh_paged_padded_dim(dim) + 4) * 4;
+uint32_t rows_kept(uint32_t tile_rows, uint32_t max_rows, uint32_t heads, uint32_t kv_heads) {
+    return tile_rows == 16 ? (uint32_t)std::min<uint64_t>(16, (uint64_t)max_rows * (heads / kv_heads)) : tile_rows;
 }
+size_t cut_bytes(const Cut& c, uint32_t kept, uint32_t kv_heads, uint32_t dim) { return (size_t)c.records * kv_heads * kept * (lh_paged_padded_dim(dim) + 4) * 4; }
 
 template <int DT, int D>
-int launch_merge(lh_context* ctx, const PagedArgs& a, const char* op) {
-    constexpr uint32_t per = 256 / (D / 4);
-    // up to eight splits are on their way at once; more of them, too, where the rows fill the chip without (64 tokens of 8 kv heads in 17 parts: 27 us by
-    // workgroups, 7 so; a token in 64 parts 4.6 by workgroups)
-    if (a.splits <= 8 || (a.splits <= 32 && (uint64_t)a.tiles * a.kv_heads * 16 >= 4096))
-        hipLaunchKernelGGL((paged_merge_kernel<DT, D, true>), dim3(a.tiles * a.kv_heads * ((16 + per - 1) / per)), dim3(256), 0, ctx->stream, a);
-    else
-        hipLaunchKernelGGL((paged_merge_kernel<DT, D, false>), dim3(a.tiles * a.kv_heads * 16), dim3(256), 0, ctx->stream, a);
-    return lh_check_launch(op);
-}
-template <int DT, int D>
-int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op, uint32_t& launches) {
+int launch_rows(lh_context* ctx, const PagedArgs& a, const Cut& c, bool tiles, const char* op, uint32_t& launches) {
     int r;
+    const uint32_t wide = (uint32_t)c.parts * a.kv_heads, joins = (uint32_t)c.joins * a.kv_heads;
+    launches = joins ? 2 : 1;
     if constexpr (DT != kF32) if (tiles) {
         constexpr uint32_t KT = tile_step(D);
         const size_t lds = (size_t)4 * KT * D * 2;
         if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_tiles_kernel<DT, D>, lds, op)) != LH_OK) return r;
-        hipLaunchKernelGGL((paged_tiles_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
-        launches = 1;
-        if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
-        launches = 2;
+        hipLaunchKernelGGL((paged_tiles_kernel<DT, D>), dim3(wide), dim3(256), lds, ctx->stream, a);
+        if ((r = lh_check_launch(op)) != LH_OK || !joins) return r;
         // (17 rows of 8 heads over 4 at position 6000, 23 parts: the whole call 16.9 us without the turns, 13.9 with them)
-        if (a.splits > 4) hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, true>), dim3(a.tiles * a.kv_heads * (D / 4)), dim3(256), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, false>), dim3(a.tiles * a.kv_heads * (D / 16)), dim3(256), 0, ctx->stream, a);
+        if (c.tiles * a.kv_heads * 4 < a.fill) hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, true>), dim3(joins * (D / 4)), dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((paged_merge_tiles_kernel<DT, D, false>), dim3(joins * (D / 16)), dim3(256), 0, ctx->stream, a);
         return lh_check_launch(op);
     }
     const size_t lds = (size_t)4 * 16 * (D + 4) * 4;
     if ((r = lh_raise_dynamic_lds(ctx, (const void*)paged_rows_kernel<DT, D>, lds, op)) != LH_OK) return r;
-    hipLaunchKernelGGL((paged_rows_kernel<DT, D>), dim3(a.tiles * a.kv_heads * a.splits), dim3(256), lds, ctx->stream, a);
-    launches = 1;
-    if ((r = lh_check_launch(op)) != LH_OK || a.splits == 1) return r;
-    launches = 2;
-    return launch_merge<DT, D>(ctx, a, op);
+    hipLaunchKernelGGL((paged_rows_kernel<DT, D>), dim3(wide), dim3(256), lds, ctx->stream, a);
+    if ((r = lh_check_launch(op)) != LH_OK || !joins) return r;
+    constexpr uint32_t per = 256 / (D / 4);
+    // (up to eight parts of most tiles are on their way at once; more take turns)
+    if (c.tiles * a.kv_heads * 8 >= a.fill) hipLaunchKernelGGL((paged_merge_kernel<DT, D, true>), dim3(joins, (a.rows_kept + per - 1) / per), dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((paged_merge_kernel<DT, D, false>), dim3(joins, a.rows_kept), dim3(256), 0, ctx->stream, a);
+    return lh_check_launch(op);
 }
 template <int DT>
-int launch_rows(lh_context* ctx, const PagedArgs& a, bool tiles, const char* op, uint32_t& launches) {
+int launch_rows(lh_context* ctx, const PagedArgs& a, const Cut& c, bool tiles, const char* op, uint32_t& launches) {
     switch (lh_paged_padded_dim(a.dim)) {
-        case 32: return launch_rows<DT, 32>(ctx, a, tiles, op, launches);
-        case 64: return launch_rows<DT, 64>(ctx, a, tiles, op, launches);
-        case 128: return launch_rows<DT, 128>(ctx, a, tiles, op, launches);
-        case 192: return launch_rows<DT, 192>(ctx, a, tiles, op, launches);
-        default: return launch_rows<DT, 256>(ctx, a, tiles, op, launches);
+        case 32: return launch_rows<DT, 32>(ctx, a, c, tiles, op, launches);
+        case 64: return launch_rows<DT, 64>(ctx, a, c, tiles, op, launches);
+        case 128: return launch_rows<DT, 128>(ctx, a, c, tiles, op, launches);
+        case 192: return launch_rows<DT, 192>(ctx, a, c, tiles, op, launches);
+        default: return launch_rows<DT, 256>(ctx, a, c, tiles, op, launches);
     }
 }
 }  // namespace
@@ -1002,8 +1073,8 @@ size_t lh_paged_attention_workspace_bytes(uint32_t rows, uint32_t sequences, uin
     size_t most = 0;                                          // of all types
     for (int dtype : {LH_BF16, LH_F32}) {
         const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
-        const uint32_t n = tiles ? 128 : 16;
-        most = std::max(most, cut_bytes(cut(n, tiles ? tile_step(lh_paged_padded_dim(dim)) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, 0), n, kv_heads, dim));
+        const uint32_t n = tiles ? 128 : 16, kept = rows_kept(n, max_rows, heads, kv_heads);
+        most = std::max(most, cut_bytes(cut(n, tiles ? tile_step(lh_paged_padded_dim(dim)) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, 0), kept, kv_heads, dim));
     }
     return most;
 }
@@ -1038,32 +1109,33 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
     const uint32_t tile_rows = tiles ? 128 : 16;
     const Cut c = cut(tile_rows, tiles ? tile_step(lh_paged_padded_dim(dim)) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, window);
-    if (c.splits > 1) {
-        const size_t bytes = cut_bytes(c, tile_rows, kv_heads, dim);
+    a.rows_kept = rows_kept(tile_rows, max_rows, heads, kv_heads);
+    if (c.records) {
+        const size_t bytes = cut_bytes(c, a.rows_kept, kv_heads, dim);
         LH_NEED(workspace, bytes, op, "workspace");
         LH_REQUIRE(paged_apart(workspace, bytes, output, out_bytes) && paged_apart(workspace, bytes, keys, pool) && paged_apart(workspace, bytes, values, pool) &&
                        paged_apart(workspace, bytes, q, ((size_t)(rows - 1) * q_ld + width) * size), "%s: workspace overlaps what the call reads or writes", op);
         LH_REQUIRE(((uintptr_t)workspace->ptr & 15) == 0, "%s: workspace has to begin at 16 bytes", op);
         a.partial = (float*)workspace->ptr;
     }
-    LH_REQUIRE(c.tiles * kv_heads * std::max(c.splits, c.splits == 1 ? 1u : 64u) <= kMaxWorkgroups, "%s: %u rows of %u heads", op, rows, heads);
+    LH_REQUIRE(std::max(c.parts, c.joins * 64) * kv_heads <= kMaxWorkgroups, "%s: %u rows of %u heads", op, rows, heads);
     a.q = q->ptr; a.keys = keys->ptr; a.values = values->ptr; a.out = output->ptr;
     a.plan = PagedPlan{(const uint32_t*)table->ptr, (const uint32_t*)starts->ptr, (const uint32_t*)lengths->ptr, rows, sequences, table_ld, pages, (uint32_t)__builtin_ctz(page)};
     a.q_ld = q_ld; a.out_ld = output_ld;
     a.max_rows = max_rows; a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.window = window;
     a.capacity = (uint32_t)std::min<uint64_t>((uint64_t)table_ld * page, max_length);
-    a.tiles = (uint32_t)c.tiles; a.splits = c.splits; a.chunk = c.chunk;
+    a.most = c.most; a.least = c.least; a.fill = c.fill; a.share = c.share; a.coarse = c.coarse; a.fixed = c.fixed; a.parts = (uint32_t)c.parts; a.records = (uint32_t)c.records;
     a.q_wide = (((uintptr_t)a.q | (uint64_t)q_ld * size | (uint64_t)dim * size) & 15) == 0;
     a.out_wide = (((uintptr_t)a.out | (uint64_t)output_ld * size | (uint64_t)dim * size) & 15) == 0;
     a.scale2 = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
     a.negative = scale < 0.0f; a.nothing = scale == 0.0f;
     a.stream = (uint64_t)sequences * max_length * kv_heads * 2 * lh_paged_padded_dim(dim) * size > (32ull << 20);
     a.q_plain = a.q_wide && scale > 0.0f && dim == lh_paged_padded_dim(dim);
-    a.group = Divisor(heads / kv_heads); a.by_heads = Divisor(kv_heads); a.by_cut = Divisor(kv_heads * c.splits); a.by_chunk = Divisor(c.chunk);
+    a.group = Divisor(heads / kv_heads); a.by_heads = Divisor(kv_heads);
     uint32_t launches = 0;
-    if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, tiles, op, launches);
-    else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, tiles, op, launches);
-    else r = launch_rows<kBf16>(batch->ctx, a, tiles, op, launches);
+    if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, c, tiles, op, launches);
+    else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, c, tiles, op, launches);
+    else r = launch_rows<kBf16>(batch->ctx, a, c, tiles, op, launches);
     batch->dispatch_count += launches;
     return r;
 }

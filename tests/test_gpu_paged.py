@@ -210,12 +210,15 @@ def run_attention(dev, step, dtype, heads, G, dim, window=0, sink=False, seed=0,
     out = dev.up(marked, lead)
     ml, mr = step.max_length if max_length is None else max_length, step.max_rows if max_rows is None else max_rows
     need = K.paged_attention_workspace_bytes(rows, len(step.sequences), mr, ml, heads, G, dim)
-    work = pkg.Buffer.empty(dev.ctx, max(need, 16))
+    whole, mark = pkg.Buffer.empty(dev.ctx, need + 256), np.arange(256, dtype=np.uint8)
+    work, behind = whole.view(0, max(need, 16)), whole.view(need, 256)
+    dev.batch().write(behind, mark)
     K.paged_attention_into(dev.batch(), dev.up(q, lead), dev.up(keys), dev.up(values), out, code(pkg, dtype), dev.up(step.table), dev.up(step.starts), dev.up(step.lengths), rows,
                            len(step.sequences), mr, ml, heads, G, dim, step.pages, step.page, step.table.shape[1], q_ld, out_ld, scale, window,
                            dev.up(s) if sink else None, work if need else None)
     got = dev.down(out, (rows, out_ld), dtype)
     assert same_bits(got[:, heads * dim:], marked[:, heads * dim:], dtype)
+    assert bool((behind.as_array(np.uint8, 256) == mark).all())
     got = got[:, :heads * dim].reshape(rows, heads, dim)
     q = q[:, :heads * dim].reshape(rows, heads, dim)
     want, tol = attended(step, q, keys, values, float(np.float32(scale)), window, s, max_length, max_rows)
@@ -394,6 +397,48 @@ def test_attention_of_sequences_with_and_without_a_common_beginning(dev, dtype, 
     step.table[4, 7] = NO_PAGE
     run_attention(dev, step, dtype, 8, 2, dim, seed=dim, max_length=40000)
     run_attention(dev, step, dtype, 8, 2, dim, 700, True, seed=dim + 1, max_length=40000)
+
+
+BOUNDS = [  # sequences (rows, length), page, heads, kv heads, dim, window
+    ([(1, 9000)] + [(1, 30 + i) for i in range(70)], 64, 8, 2, 64, 0),               # one long among many short ones
+    ([(1, 700)] * 3, 16, 4, 4, 128, 0),
+    ([(60, 5000), (60, 60), (1, 2000), (3, 3)], 32, 8, 2, 64, 0),
+    ([(200, 200)] * 20 + [(130, 3000)], 32, 8, 8, 32, 0),                             # tiles that fill the chip
+    ([(5, 4000)] * 9, 64, 6, 2, 192, 1500),
+    ([(1, 40)] * 300, 16, 16, 16, 32, 0),                                             # more units than workgroups are wanted
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(BOUNDS)))
+@pytest.mark.parametrize("bound", [1, 9, 300])
+def test_attention_of_a_call_for_longer_sequences(dev, dtype, case, bound):
+    """How sequences are cut goes by what they have, not by what the call allows."""
+    seqs, page, heads, G, dim, window = BOUNDS[case]
+    step = Step(seqs, page, seed=case)
+    run_attention(dev, step, dtype, heads, G, dim, window, sink=case % 2 == 1, seed=case, max_length=step.max_length * bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 60])
+def test_attention_of_starts_that_do_not_ascend(dev, dtype, rows):
+    """What such a step computes is not said, but it stays inside its buffers: more tiles and parts than the rows can have are left out."""
+    pkg, K = dev.pkg, dev.K
+    n, G, D, page, length = 40, 2, 64, 64, 6000
+    step = Step([(rows, length)], page, seed=rows)
+    table, lengths = np.repeat(step.table, n, 0), np.full(n, length, np.uint32)
+    starts = np.zeros(n + 1, np.uint32)
+    starts[1::2] = rows                                            # every other sequence has all the rows
+    keys, values = (dev.up(normal(i, step.pages, G, page, D, dtype=dtype)) for i in range(2))
+    q, marked = normal(2, rows, 8 * D, dtype=dtype), torch.full((rows + 1, 8 * D), 7.0).to(TYPES[dtype])
+    need = K.paged_attention_workspace_bytes(rows, n, rows, length, 8, G, D)
+    whole, mark, out = pkg.Buffer.empty(dev.ctx, need + 256), np.arange(256, dtype=np.uint8), dev.up(marked)
+    dev.batch().write(whole.view(need, 256), mark)
+    K.paged_attention_into(dev.batch(), dev.up(q), keys, values, out, code(pkg, dtype), dev.up(table), dev.up(starts), dev.up(lengths), rows, n, rows, length, 8, G, D,
+                           step.pages, page, table.shape[1], 8 * D, 8 * D, 0.1, 0, None, whole.view(0, need))
+    got = dev.down(out, (rows + 1, 8 * D), dtype)
+    assert same_bits(got[rows:], marked[rows:], dtype)
+    assert bool((whole.view(need, 256).as_array(np.uint8, 256) == mark).all())
 
 
 def test_attention_of_no_sequence_and_of_one_that_ends_behind_the_rows(dev):
