@@ -324,8 +324,8 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint6
 //                  pairs of positions are put together in registers, a column per product: no LDS on the way
 // Weights of 16 bits are two terms, what the first leaves being the second: the products are few beside the loads, and what a result is off
 // stays that of its own rounding.
-// Memory binds it: 64 tokens over 4096 to 16384 positions of 8 kv heads of 128 (2.6 GB in pages of 16 positions, runs of 4 KB) 434 us, 6.0 TB/s,
-// where reading alone reaches 6.2 to 6.8 in runs of 8 KB; 15 % of a SIMD's time is vector and matrix work.  One token over 32768 (134 MB) 23 us.
+// Memory binds it: 64 tokens over 4096 to 16384 positions of 8 kv heads of 128 (2.6 GB in pages of 16 positions, runs of 4 KB) 421 us, 6.2 TB/s,
+// where reading alone reaches 6.2 to 6.8 in runs of 8 KB; 15 % of a SIMD's time is vector and matrix work.  One token over 32768 (134 MB) 24 us.
 // The next step's keys are requested when this one's are used, its values likewise (the 64 tokens 450 -> 444 us).
 // The hint that nothing is read again, for caches that would push everything else out from near the chip: 472 -> 450, the token with its pages in memory
 // 31.9 -> 28.9 (where the last launch has left them near, 26.9 -> 27.3).  Pages that sequences share are read again, and soon: 64 tokens over the same 16384
