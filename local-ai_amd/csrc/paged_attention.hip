@@ -78,34 +78,40 @@ __device__ __forceinline__ uint32_t whole(uint32_t n, uint32_t d) {
 struct Load { uint32_t first, all, length, tiles, steps; };
 template <uint32_t ROWS, uint32_t STEP>
 __device__ __forceinline__ Load load_of(const PagedArgs& a, uint32_t s) {
-    Load c{0, 0, 0, 0, 0};
-    if (s < a.plan.sequences) {
-        c.first = a.plan.starts[s];
-        c.length = a.plan.lengths[s];
-        const uint32_t end = a.plan.starts[s + 1];
-        if (end > c.first && end <= a.plan.rows) {
-            c.all = end - c.first;
-            c.tiles = (uint32_t)(((uint64_t)min(c.all, a.max_rows) * a.group.d + ROWS - 1) / ROWS);
-            c.steps = min((min(c.length, a.capacity) + STEP - 1) / STEP, a.most);
-        }
-    }
+    Load c;
+    const uint32_t some = min(s, a.plan.sequences - 1);       // (loads without branches go out together)
+    c.first = a.plan.starts[some];
+    c.length = a.plan.lengths[some];
+    const uint32_t end = a.plan.starts[some + 1];
+    const bool on = s < a.plan.sequences && end > c.first && end <= a.plan.rows;
+    c.all = on ? end - c.first : 0u;
+    c.tiles = (uint32_t)(((uint64_t)min(c.all, a.max_rows) * a.group.d + ROWS - 1) / ROWS);
+    c.steps = on ? min((min(c.length, a.capacity) + STEP - 1) / STEP, a.most) : 0u;
     return c;
 }
 
 // Steps of a part: what all tiles have to do over the workgroups wanted, so that a long sequence among short ones is cut and short ones alone are not, whatever bound the
 // call gives for their lengths (64 tokens at 4000 of a call for up to 131072: parts by the bound 313 us, so 171; 256 at 1000 653 and 174).  Where there are few tiles,
-// equal ones make a whole number of parts.  It costs every workgroup two scans and a reciprocal, 0.5 us.  All kernels of a call find the same.
+// equal ones make a whole number of parts.  It costs every workgroup two scans and a reciprocal, 0.2 us, and 5 with a thousand sequences (1024 at 1000 in a call for up to 16384
+// 658 -> 694 us).  All kernels of a call find the same.
 //   The sum is of steps shifted by `coarse` and rounded up, which lets it fit.  The chunk is at least what all have over `share`: so the parts of all tiles are at most
 //   `share` more than there are tiles, and, a tile in parts having more than a chunk, those of such tiles at most twice `share`.
 template <uint32_t ROWS, uint32_t STEP>
-__device__ __forceinline__ uint32_t chunk_of(const PagedArgs& a, uint32_t lane, Load& c) {
+__device__ __forceinline__ uint32_t chunk_of(const PagedArgs& a, uint32_t lane, Load& c, uint32_t& longest) {
+    if (a.fixed) {
+        if (a.plan.sequences <= 64) c = load_of<ROWS, STEP>(a, lane);
+        longest = a.most;
+        return a.least;
+    }
     uint32_t tiles = 0, work = 0;
+    longest = 0;
+#pragma unroll 4
     for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 64) {
         c = load_of<ROWS, STEP>(a, s0 + lane);
         tiles += c.tiles;
+        longest = max(longest, c.steps);
         work += (uint32_t)(((uint64_t)c.tiles * c.steps + (1ull << a.coarse) - 1) >> a.coarse);
     }
-    if (a.fixed) return a.least;
     tiles = __builtin_amdgcn_readlane(sum_up_to(tiles), 63);
     work = __builtin_amdgcn_readlane(sum_up_to(work), 63);
     const uint64_t units = (uint64_t)tiles * a.kv_heads;
@@ -133,32 +139,42 @@ template <uint32_t ROWS, uint32_t STEP, bool JOIN>
 __device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t n, uint32_t lane) {
     const uint32_t R = a.group.d;
     Tile r{-1, 0, 0, 0, 0, 0, 1, 0, 0};
-    Load c;
-    r.chunk = chunk_of<ROWS, STEP>(a, lane, c);
-    uint32_t before = 0, records = 0;
-    for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 64) {
-        if (a.plan.sequences > 64) c = load_of<ROWS, STEP>(a, s0 + lane);
+    Load own;
+    uint32_t longest, before = 0, records = 0;
+    r.chunk = chunk_of<ROWS, STEP>(a, lane, own, longest);
+    if (JOIN && !__any(longest > r.chunk)) return r;
+    // whether it is of the 64 sequences from s0 on
+    const auto found = [&](const Load& c, uint32_t s0) __attribute__((always_inline)) {
         const uint32_t parts = max(about(c.steps + r.chunk - 1, r.chunk), 1u), all = c.tiles * parts, kept = parts > 1 ? all : 0u, size = JOIN ? (parts > 1 ? c.tiles : 0u) : all;
         const uint32_t sum = sum_up_to(size), kept_sum = sum_up_to(kept);
         const uint64_t behind = __ballot(before + sum > n);
-        if (behind) {
-            const int at = __builtin_ctzll(behind);
-            const uint32_t brought = __builtin_amdgcn_readlane(c.all, at), rows = min(brought, a.max_rows) * R;
-            r.sequence = s0 + at;
-            r.first = __builtin_amdgcn_readlane(c.first, at);
-            r.parts = __builtin_amdgcn_readlane(parts, at);
-            const uint32_t in = n - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(size, at)), tiles = __builtin_amdgcn_readlane(c.tiles, at);
-            r.split = JOIN || r.parts == 1 ? 0u : whole(in, tiles);
-            const uint32_t i = in - r.split * tiles;
-            r.record = records + (__builtin_amdgcn_readlane(kept_sum, at) - __builtin_amdgcn_readlane(kept, at)) + i * r.parts;
-            if (i >= tiles || (r.parts > 1 && r.record + r.parts > a.records)) r.sequence = -1;      // (only where starts do not ascend: the sums say nothing then)
-            r.row0 = i * ROWS;
-            r.count = min(ROWS, rows - r.row0);
-            r.begin = (int64_t)(uint32_t)__builtin_amdgcn_readlane(c.length, at) - brought;
-            return r;
+        if (!behind) {
+            before += __builtin_amdgcn_readlane(sum, 63);
+            records += __builtin_amdgcn_readlane(kept_sum, 63);
+            return false;
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
-        records += __builtin_amdgcn_readlane(kept_sum, 63);
+        const int at = __builtin_ctzll(behind);
+        const uint32_t brought = __builtin_amdgcn_readlane(c.all, at), rows = min(brought, a.max_rows) * R;
+        r.sequence = s0 + at;
+        r.first = __builtin_amdgcn_readlane(c.first, at);
+        r.parts = __builtin_amdgcn_readlane(parts, at);
+        const uint32_t in = n - before - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(size, at)), tiles = __builtin_amdgcn_readlane(c.tiles, at);
+        r.split = JOIN || r.parts == 1 ? 0u : whole(in, tiles);
+        const uint32_t i = in - r.split * tiles;
+        r.record = records + (__builtin_amdgcn_readlane(kept_sum, at) - __builtin_amdgcn_readlane(kept, at)) + i * r.parts;
+        if (i >= tiles || (r.parts > 1 && r.record + r.parts > a.records)) r.sequence = -1;      // (only where starts do not ascend: the sums say nothing then)
+        r.row0 = i * ROWS;
+        r.count = min(ROWS, rows - r.row0);
+        r.begin = (int64_t)(uint32_t)__builtin_amdgcn_readlane(c.length, at) - brought;
+        return true;
+    };
+    if (a.plan.sequences <= 64) {
+        found(own, 0);
+        return r;
+    }
+    for (uint32_t s0 = 0; s0 < a.plan.sequences; s0 += 256) {
+        const Load c[4] = {load_of<ROWS, STEP>(a, s0 + lane), load_of<ROWS, STEP>(a, s0 + 64 + lane), load_of<ROWS, STEP>(a, s0 + 128 + lane), load_of<ROWS, STEP>(a, s0 + 192 + lane)};
+        if (found(c[0], s0) || found(c[1], s0 + 64) || found(c[2], s0 + 128) || found(c[3], s0 + 192)) return r;
     }
     return r;
 }
