@@ -37,7 +37,7 @@ struct PagedArgs {
     const void *q, *keys, *values;
     void* out;
     const float* sink;         // [heads], may be null
-    float* partial;            // records [tile][kv head][split] of (D + 4) values a row: unnormalised sums, maximum, sum of weights
+    float* partial;            // records of (D + 4) values a row, a part's by Tile::record_of: unnormalised sums, maximum, sum of weights
     PagedPlan plan;
     uint64_t q_ld, out_ld;
     uint32_t max_rows, heads, kv_heads, dim, window, capacity;     // capacity: positions from there on are not seen
