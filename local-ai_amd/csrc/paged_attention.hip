@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? (D <= 128 ? 2 : 1) : D <= 128 ? 3
         for (int w = 0; w < 4; w++) {
             const lh_f32x4 y = *reinterpret_cast<const lh_f32x4*>(slab + (w * 16 + r) * kRow + c);
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] += f[w] == 0.0f ? 0.0f : f[w] * y[j];
+            for (int j = 0; j < 4; j++) x[j] += f[w] * y[j];      // (a NaN that weighs nothing is one all the same; a wave that saw nothing has zeros)
         }
         if (rec) { *reinterpret_cast<lh_f32x4*>(rec + c) = x; continue; }
 #pragma unroll
@@ -878,7 +878,7 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs 
         float nm = m;
 #pragma unroll
         for (uint32_t i = 0; i < n; i++) {
-            if (st[i].y == 0.0f) { st[i].x = -INFINITY; p[i] = q[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f}; }      // nothing seen there
+            if (st[i].y == 0.0f) st[i].x = -INFINITY;          // nothing that weighs anything: zeros, or a NaN that was seen
             nm = fmaxf(nm, st[i].x);
         }
         const float zero = nm == -INFINITY ? 0.0f : nm, before = __builtin_amdgcn_exp2f(m - zero);
@@ -906,7 +906,7 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(const PagedArgs 
             st[i] = reinterpret_cast<const float2*>(from + 128 * D)[r];
         }
 #pragma unroll
-        for (uint32_t i = 0; i < BATCH; i++) if (s0 + i * each >= part.used) st[i].y = 0.0f;
+        for (uint32_t i = 0; i < BATCH; i++) if (s0 + i * each >= part.used) { st[i].y = 0.0f; p[i] = q[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f}; }
         join(st, p, q, std::integral_constant<uint32_t, BATCH>());
     }
     if constexpr (MANY) {
@@ -960,7 +960,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
         float nm = m;
 #pragma unroll
         for (uint32_t i = 0; i < BATCH; i++) {
-            if (s0 + i * each >= part.used || st[i].y == 0.0f) { st[i] = make_float2(-INFINITY, 0.0f); y[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f}; }    // nothing seen there
+            if (s0 + i * each >= part.used) { st[i].y = 0.0f; y[i] = (lh_f32x4){0.f, 0.f, 0.f, 0.f}; }
+            if (st[i].y == 0.0f) st[i].x = -INFINITY;          // nothing that weighs anything: zeros, or a NaN that was seen
             nm = fmaxf(nm, st[i].x);
         }
         const float zero = nm == -INFINITY ? 0.0f : nm, before = __builtin_amdgcn_exp2f(m - zero);

@@ -613,3 +613,49 @@ def test_a_recorded_step_follows_its_plan(dev, dtype, rows):
             assert same_bits(got, dev.down(s.other, (n, H, dim), dtype), dtype) and same_bits(turned, dev.down(s.out, (n, H, dim), dtype), dtype)
             for a, b in zip(s.pools, s.twin):
                 assert same_bits(dev.down(a, shape, dtype), dev.down(b, shape, dtype), dtype)
+
+
+# ---- values that are seen, however little they weigh ---------------------------------------------------------------------------
+def attention_of(dev, step, q, keys, values, dtype, scale, window=0, sink=None, max_length=None):
+    pkg, K = dev.pkg, dev.K
+    rows, H, dim = q.shape
+    G, ml = keys.shape[1], step.max_length if max_length is None else max_length
+    out = pkg.Buffer.empty(dev.ctx, q.numel() * q.element_size())
+    need = K.paged_attention_workspace_bytes(rows, len(step.sequences), step.max_rows, ml, H, G, dim)
+    K.paged_attention_into(dev.batch(), dev.up(q), dev.up(keys), dev.up(values), out, code(pkg, dtype), dev.up(step.table), dev.up(step.starts), dev.up(step.lengths), rows,
+                           len(step.sequences), step.max_rows, ml, H, G, dim, step.pages, step.page, step.table.shape[1], H * dim, H * dim, scale, window,
+                           None if sink is None else dev.up(sink), pkg.Buffer.empty(dev.ctx, max(need, 16)))
+    return dev.down(out, q.shape, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("length,at", [(400, 20), (400, 300), (6000, 20), (6000, 150), (6000, 3000), (6000, 5900)])
+@pytest.mark.parametrize("weight", ["key", "sink", "none"])
+def test_a_nan_that_a_row_sees_reaches_it(dev, dtype, rows, length, at, weight):
+    """A NaN among the values of a position beside which another (or the sink) weighs 2^230 times as much, or whose score is minus infinity as those of all positions near
+    it are: 0 times NaN is NaN, whichever wave or part has the position.
+
+    Tolerance: a weight below 2^-126 may be 0, which 6000 of them times values of at most 5 make less than 2^-110 of."""
+    G, dim = 2, 64
+    step = Step([(rows, length)], 32, seed=length)
+    shape = (step.pages, G, 32, dim)
+    keys, values = torch.zeros(shape, dtype=TYPES[dtype]), normal(1, *shape, dtype=dtype)
+
+    def place(p):
+        return int(step.table[0, p // 32]), p % 32
+    sink = torch.full((4,), 160.0) if weight == "sink" else None
+    if weight == "key":
+        keys[place(5)[0], :, place(5)[1], 0] = 160.0
+    if weight == "none":
+        keys[..., 0] = -math.inf
+        keys[place(5)[0], :, place(5)[1], 0] = 0.0
+    values[place(at)[0], 1, place(at)[1], 7] = math.nan
+    q = torch.zeros(rows, 4, dim, dtype=TYPES[dtype])
+    q[..., 0] = 1.0
+    got = attention_of(dev, step, q, keys, values, dtype, 1.0, sink=sink)
+    want, tol = attended(step, q, keys, values, 1.0, sink=sink)
+    assert bool(want[:, 2:, 7].isnan().all()) and int(want.isnan().sum()) == 2 * rows
+    if weight == "none":                                           # (one position has all the weight: 1, exactly)
+        tol = torch.zeros_like(tol)
+    close(got, want, half_step(dtype) * want.abs() + tol + (2.0 ** -25 if dtype == "f16" else 2.0 ** -110))
