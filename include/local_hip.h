@@ -924,7 +924,8 @@ LH_API int lh_moe_vector_down_into(lh_batch* batch, const lh_buffer* hidden, con
  *                `fast` turns in `original` positions stay, those that make at most `slow` are divided, the ones between shade over
  *                (NTK by parts, "YaRN": Peng et al., 2023), and *amplitude is 0.1 ln(factor) + 1 (else 1)
  *   rows         input and output rows of [heads, dim], input_ld and output_ld values apart; LH_F16, LH_BF16 or LH_F32; positions u32
- *                [rows] in device memory.  Output may be the input (same buffer, same distance) and may not overlap it otherwise. */
+ *                [rows] in device memory.  Output may be the input (same buffer, same distance) and may not overlap it otherwise, nor positions or
+ *                frequencies (between two of its rows there is room for others' data). */
 #define LH_ROTARY_PAIRS 0
 #define LH_ROTARY_HALVES 1
 #define LH_ROTARY_PLAIN 0
@@ -945,7 +946,8 @@ LH_API int lh_rotary_rows_into(lh_batch* batch, const lh_buffer* input, lh_buffe
  *   lengths  [sequences]: positions of a sequence with its rows in; its last row stands at lengths[s] - 1.  Rows before position 0,
  *            where a sequence has more rows than positions, stand nowhere.
  * What a table says of pages that the pool does not have, and positions that the table does not reach, are dropped when written and not
- * seen when read; rows of no sequence are left as they were, and so are those of one that ends behind `rows`.
+ * seen when read; rows of no sequence are left as they were, and so are those of one that ends behind `rows`.  What a call writes may not lie
+ * over what it reads, its workspace included; q_output and q below are the one exception.
  *   append     k and v rows [kv_heads, dim], k_ld and v_ld values apart, go to their pages, k turned as in lh_rotary_rows_into; the
  *              columns behind dim become zero.  q (may be null, with heads 0) is turned by the same positions into q_output, which may be
  *              q (a row that stands nowhere is left out).  frequencies may be null with rot 0: nothing turns.  No two sequences append to

@@ -87,5 +87,21 @@ inline bool paged_rows_meet(const lh_buffer* a, uint64_t awidth, uint32_t ald, c
     const size_t ld = (size_t)ald * size, d = b0 >= a0 ? (b0 - a0) % ld : (ld - (a0 - b0) % ld) % ld;    // where b's row begins in a's
     return d < awidth * size || d + bwidth * size > ld;
 }
+// Whether `bytes` at the start of b share memory with rows of `width` bytes, `ld` bytes apart, from `out` on.
+inline bool paged_meets(const lh_buffer* b, size_t bytes, const lh_buffer* out, size_t width, size_t ld, uint32_t rows) {
+    if (bytes == 0 || rows == 0 || width == 0) return false;
+    const uintptr_t b0 = (uintptr_t)b->ptr, o0 = (uintptr_t)out->ptr;
+    if (b0 + bytes <= o0 || o0 + (size_t)(rows - 1) * ld + width <= b0) return false;
+    if (b0 < o0) return true;
+    const size_t at = (b0 - o0) % ld;                         // between two rows there is room for others' data
+    return at < width || at + bytes > ld;
+}
+// What a step's plan is read from, beside the rows: none of it may lie where a kernel writes.
+struct PagedRead { const lh_buffer* b; size_t bytes; const char* name; };
+template <size_t N>
+inline int paged_need_apart(const char* op, const PagedRead (&read)[N], const lh_buffer* out, const char* name, size_t width, size_t ld, uint32_t rows) {
+    for (const PagedRead& r : read) LH_REQUIRE(!r.b || !paged_meets(r.b, r.bytes, out, width, ld, rows), "%s: %s lies over %s", op, name, r.name);
+    return LH_OK;
+}
 
 }  // namespace

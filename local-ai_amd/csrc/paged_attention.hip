@@ -1123,6 +1123,9 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
         LH_REQUIRE(((uintptr_t)sink->ptr & 3) == 0, "%s: sink has to begin at 4 bytes", op);
         a.sink = (const float*)sink->ptr;
     }
+    const PagedRead read[] = {{table, (size_t)sequences * table_ld * 4, "table"}, {starts, ((size_t)sequences + 1) * 4, "starts"}, {lengths, (size_t)sequences * 4, "lengths"},
+                              {sink, (size_t)heads * 4, "sink"}};
+    if ((r = paged_need_apart(op, read, output, "output", width * size, (size_t)output_ld * size, rows)) != LH_OK) return r;
     const bool tiles = takes_tiles(dtype, max_rows, heads, kv_heads);
     const uint32_t tile_rows = tiles ? 128 : 16;
     const Cut c = cut(tile_rows, tiles ? tile_step(lh_paged_padded_dim(dim)) : 32, dim, rows, sequences, max_rows, max_length, heads, kv_heads, window);
@@ -1132,6 +1135,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
         LH_NEED(workspace, bytes, op, "workspace");
         LH_REQUIRE(paged_apart(workspace, bytes, output, out_bytes) && paged_apart(workspace, bytes, keys, pool) && paged_apart(workspace, bytes, values, pool) &&
                        paged_apart(workspace, bytes, q, ((size_t)(rows - 1) * q_ld + width) * size), "%s: workspace overlaps what the call reads or writes", op);
+        if ((r = paged_need_apart(op, read, workspace, "workspace", bytes, bytes, 1)) != LH_OK) return r;
         LH_REQUIRE(((uintptr_t)workspace->ptr & 15) == 0, "%s: workspace has to begin at 16 bytes", op);
         a.partial = (float*)workspace->ptr;
     }

@@ -257,6 +257,8 @@ int lh_rotary_rows_into(lh_batch* batch, const lh_buffer* input, lh_buffer* outp
     LH_REQUIRE(((uintptr_t)positions->ptr & 3) == 0, "%s: positions have to begin at 4 bytes", op);
     LH_REQUIRE((input->ptr == output->ptr && input_ld == output_ld) || !paged_rows_meet(input, width, input_ld, output, width, output_ld, rows, size),
                "%s: input and output overlap and are not the same", op);
+    const PagedRead read[] = {{positions, (size_t)rows * 4, "positions"}, {frequencies, (size_t)rot / 2 * 4, "frequencies"}};
+    if ((r = paged_need_apart(op, read, output, "output", width * size, (size_t)output_ld * size, rows)) != LH_OK) return r;
     TurnArgs a{};
     a.in = input->ptr; a.out = output->ptr; a.in_ld = input_ld; a.out_ld = output_ld;
     a.heads = heads; a.dim = dim; a.rot = rot; a.first = first; a.rows = rows; a.padded = dim;
@@ -298,6 +300,11 @@ int lh_paged_append_into(lh_batch* batch, const lh_buffer* k, const lh_buffer* v
     for (const lh_buffer* p : {(const lh_buffer*)keys, (const lh_buffer*)values})
         LH_REQUIRE(apart(k, kvw, k_ld, p) && apart(v, kvw, v_ld, p) && (!q || (apart(q, qw, q_ld, p) && apart(q_output, qw, q_output_ld, p))), "%s: the rows lie inside the pages", op);
     LH_REQUIRE(paged_apart(keys, pool, values, pool), "%s: keys and values have pages of their own", op);
+    const PagedRead read[] = {{table, (size_t)sequences * table_ld * 4, "table"}, {starts, ((size_t)sequences + 1) * 4, "starts"}, {lengths, (size_t)sequences * 4, "lengths"},
+                              {frequencies, (size_t)rot / 2 * 4, "frequencies"}};
+    if ((r = paged_need_apart(op, read, keys, "keys", pool, pool, 1)) != LH_OK) return r;
+    if ((r = paged_need_apart(op, read, values, "values", pool, pool, 1)) != LH_OK) return r;
+    if (q && (r = paged_need_apart(op, read, q_output, "q_output", qw * size, (size_t)q_output_ld * size, rows)) != LH_OK) return r;
     TurnArgs a{};
     if (q) { a.in = q->ptr; a.out = q_output->ptr; a.in_ld = q_ld; a.out_ld = q_output_ld; }
     a.heads = heads; a.dim = dim; a.rot = rot; a.first = rot ? first : 0; a.rows = rows;

@@ -659,3 +659,18 @@ def test_a_nan_that_a_row_sees_reaches_it(dev, dtype, rows, length, at, weight):
     if weight == "none":                                           # (one position has all the weight: 1, exactly)
         tol = torch.zeros_like(tol)
     close(got, want, half_step(dtype) * want.abs() + tol + (2.0 ** -25 if dtype == "f16" else 2.0 ** -110))
+
+
+def test_what_is_read_may_stand_between_the_rows_of_an_output(dev):
+    """One allocation: rows of 64 values, 128 apart, with the frequencies behind the first and the positions behind the second."""
+    pkg, K = dev.pkg, dev.K
+    rows, ld = 3, 128
+    x, f, at = normal(1, rows, 64), K.rotary_frequencies(64, 1e4)[0], np.asarray([7, 100, 3000], np.uint32)
+    whole = torch.full((rows, ld), 7.0)
+    whole[0, 64:96], whole[1, 64:67] = torch.from_numpy(f), torch.from_numpy(at.view(np.float32))
+    b = dev.up(whole)
+    K.rotary_rows_into(dev.batch(), dev.up(x), b, pkg.F32, b.view(4 * (ld + 64), 12), b.view(4 * 64, 128), 1.0, rows, 1, 64, 64, 0, pkg.ROTARY_HALVES, 64, ld)
+    got = dev.down(b, (rows, ld), "f32")
+    want, sizes = turn(x.reshape(rows, 1, 64), at, f, 1.0, 64, 0, True)
+    close(got[:, :64].reshape(rows, 1, 64), want, turn_tolerance(want, sizes, "f32"))
+    assert same_bits(got[:, 64:], whole[:, 64:], "f32")

@@ -241,3 +241,40 @@ def test_attention_refusals(pkg):
                     dict(output=buf(4 * GB + pool - 2, 6 * 800 * 2)), dict(workspace=buf(2 * GB + 6 * 1600 - 16, need)), dict(workspace=buf(GB - need + 16, need)),
                     dict(workspace=buf(3 * GB + 16, need))):
         c.refused(**changed)
+
+
+# ---- what is read may not lie where a call writes ----------------------------------------------------------------------------------
+def test_rotary_outputs_over_what_is_read_are_refused(pkg):
+    rows, ld = 10, 1024
+    c = Call(pkg, "lh_rotary_rows_into", batch=True, input=buf(GB, rows * 512 * 2), output=buf(2 * GB, rows * ld * 2), dtype=2, positions=buf(3 * GB, 40), frequencies=buf(4 * GB, 256),
+             amplitude=1.0, rows=rows, heads=4, dim=128, rot=128, first=0, pairing=1, input_ld=512, output_ld=ld)
+    for at in (2 * GB, 2 * GB - 36, 2 * GB + 9 * ld * 2 + 1020, 2 * GB + 4 * ld * 2 - 4, 2 * GB + 1000):
+        c.refused(positions=buf(at, 40))
+        assert "output lies over positions" in pkg.lib().lh_last_error().decode()
+    for at in (2 * GB, 2 * GB - 252, 2 * GB + 9 * ld * 2 + 1020, 2 * GB + ld * 2 + 1000, 2 * GB + ld * 2 - 252):
+        c.refused(frequencies=buf(at, 256))
+        assert "output lies over frequencies" in pkg.lib().lh_last_error().decode()
+
+
+def test_append_outputs_over_what_is_read_are_refused(pkg):
+    pool = 7 * 2 * 16 * 128 * 2
+    c = append_call(pkg)
+    sizes = {"table": 48, "starts": 16, "lengths": 12, "frequencies": 200}
+    for name, n in sizes.items():
+        for written, (at, end) in {"keys": (3 * GB, 3 * GB + pool), "values": (4 * GB, 4 * GB + pool), "q_output": (10 * GB, 10 * GB + 6 * 1600)}.items():
+            for where in (at - n + 4, at, (at + end) // 2 // 16 * 16, end - 4):
+                c.refused(**{name: buf(where, n)})
+                assert f"{written} lies over {name}" in pkg.lib().lh_last_error().decode()
+
+
+def test_attention_outputs_over_what_is_read_are_refused(pkg):
+    pool = 2000 * 2 * 16 * 128 * 2
+    need = pkg.lib().lh_paged_attention_workspace_bytes(6, 3, 4, 16000, 8, 2, 100)
+    c = Call(pkg, "lh_paged_attention_into", batch=True, q=buf(GB, 6 * 800 * 2), keys=buf(3 * GB, pool), values=buf(4 * GB, pool), output=buf(2 * GB, 6 * 800 * 2), dtype=2,
+             table=buf(5 * GB, 3 * 1000 * 4), starts=buf(6 * GB, 16), lengths=buf(7 * GB, 12), rows=6, sequences=3, max_rows=4, max_length=16000, heads=8, kv_heads=2, dim=100,
+             pages=2000, page=16, table_ld=1000, q_ld=800, output_ld=800, scale=0.1, window=0, sink=buf(8 * GB, 32), workspace=buf(9 * GB, need))
+    for name, n in {"table": 12000, "starts": 16, "lengths": 12, "sink": 32}.items():
+        for written, (at, end) in {"output": (2 * GB, 2 * GB + 6 * 1600), "workspace": (9 * GB, 9 * GB + need)}.items():
+            for where in (at - n + 4, at, (at + end) // 2 // 16 * 16, end - 4):
+                c.refused(**{name: buf(where, n)})
+                assert f"{written} lies over {name}" in pkg.lib().lh_last_error().decode()
