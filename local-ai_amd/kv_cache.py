@@ -338,7 +338,7 @@ class PageTables:
 
     def share(self, source: int, target: int, positions: int) -> int:
         """Gives an empty sequence the whole pages of the source's first `positions` positions; returns how many positions those hold.  What
-        stands there must be written already: neither sequence may append to them."""
+        stands there must be written already: neither sequence may append to them (``PagedStep.write`` refuses it)."""
         if self.held[target]:
             raise InvalidArgument(f"sequence {target} has pages")
         n = min(positions // self.page, self.held[source])
@@ -363,24 +363,30 @@ class PagedStep:
     def __init__(self, ctx, tables: PageTables, rows: int, max_rows: int, max_length: int):
         self.tables, self.sequences, self.table_ld = tables, *tables.table.shape
         self.rows, self.max_rows, self.max_length = rows, min(max_rows, rows), max_length
+        self.appends = True
         self.table = Buffer.empty(ctx, tables.table.nbytes)
         self.starts = Buffer.empty(ctx, 4 * (self.sequences + 1))
         self.lengths = Buffer.empty(ctx, 4 * self.sequences)
 
-    def write(self, batch, counts: Sequence[int], lengths: Sequence[int]) -> None:
-        """Sequence s brings counts[s] rows (0: it takes no part) and has lengths[s] positions with them."""
+    def write(self, batch, counts: Sequence[int], lengths: Sequence[int], append: bool = True) -> None:
+        """Sequence s brings counts[s] rows (0: it takes no part) and has lengths[s] positions with them.  Rows that will be appended may not
+        stand on pages that another sequence holds, too; without `append` the step is for attention alone, over what is there."""
         if len(counts) != self.sequences or len(lengths) != self.sequences:
             raise InvalidArgument(f"{len(counts)} and {len(lengths)} sequences of {self.sequences}")
-        for n, length, held in zip(counts, lengths, self.tables.held):
+        page = self.tables.page
+        for s, (n, length, held) in enumerate(zip(counts, lengths, self.tables.held)):
             if n < 0 or n > min(self.max_rows, length):
                 raise InvalidArgument(f"{n} rows of a sequence of {length} positions, at most {self.max_rows} in a step")
-            if n and (length > self.max_length or length > held * self.tables.page):
-                raise InvalidArgument(f"{length} positions in {held} pages of {self.tables.page}, at most {self.max_length} in a step")
+            if n and (length > self.max_length or length > held * page):
+                raise InvalidArgument(f"{length} positions in {held} pages of {page}, at most {self.max_length} in a step")
+            if n and append and (self.tables.holders[self.tables.table[s, (length - n) // page:(length - 1) // page + 1]] > 1).any():
+                raise InvalidArgument(f"sequence {s} would append positions {length - n} to {length - 1} to pages that are shared")
         if sum(counts) > self.rows:
             raise InvalidArgument(f"{sum(counts)} rows, the step was made for {self.rows}")
         batch.write(self.table, self.tables.table)
         batch.write(self.starts, np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32))
         batch.write(self.lengths, np.asarray(lengths, np.uint32))
+        self.appends = append
 
 
 @dataclass
@@ -407,6 +413,8 @@ class PagedKvCache:
                     q_output_ld: int = 0) -> None:
         """The step's keys, turned, and values to their pages; its queries turned into `q_output` (may be `q`).  Rows without a distance lie
         one behind the other."""
+        if not step.appends:
+            raise InvalidArgument("the step was written without append")
         n, h = self.kv_heads * self.dim, heads * self.dim
         turn = (rotary.frequencies, rotary.amplitude, rotary.rot, rotary.first, rotary.pairing) if rotary else ()
         kernels.paged_append_into(batch, k, v, self.dtype, self.keys, self.values, step.table, step.starts, step.lengths, step.rows, step.sequences,

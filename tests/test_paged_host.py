@@ -278,3 +278,71 @@ def test_attention_outputs_over_what_is_read_are_refused(pkg):
             for where in (at - n + 4, at, (at + end) // 2 // 16 * 16, end - 4):
                 c.refused(**{name: buf(where, n)})
                 assert f"{written} lies over {name}" in pkg.lib().lh_last_error().decode()
+
+
+# ---- steps over shared pages ---------------------------------------------------------------------------------------------------------
+class Written:
+    """Stands for a batch: what was written, no device."""
+    def __init__(self):
+        self.all = []
+
+    def write(self, dst, src):
+        self.all.append(np.array(src))
+
+
+@pytest.fixture
+def no_device(pkg, monkeypatch):
+    from local_ai_amd import kv_cache
+
+    class Fake:
+        @staticmethod
+        def empty(ctx, n):
+            return n
+    monkeypatch.setattr(kv_cache, "Buffer", Fake)
+    return kv_cache
+
+
+def test_steps_that_append_to_shared_pages_are_refused(pkg, no_device):
+    t = no_device.PageTables(12, 16, 3, 96)
+    t.reserve(0, 40)
+    assert t.share(0, 1, 40) == 32
+    t.reserve(1, 60)
+    s, b = no_device.PagedStep(None, t, rows=40, max_rows=40, max_length=96), Written()
+    for counts, lengths in (([0, 4, 0], [40, 30, 0]),                  # the target, inside what it was given
+                            ([0, 1, 0], [0, 32, 0]), ([0, 2, 0], [0, 33, 0]), ([0, 40, 0], [0, 60, 0]),
+                            ([1, 0, 0], [20, 0, 0]),                   # the source, whose pages were given away before they were written
+                            ([9, 0, 0], [40, 0, 0])):
+        with pytest.raises(pkg.InvalidArgument, match="shared"):
+            s.write(b, counts, lengths)
+        assert not b.all                                              # nothing of it is sent
+    s.write(b, [8, 28, 0], [40, 60, 0])                               # both behind what they share
+    assert [w.tolist() for w in b.all[1:]] == [[0, 8, 36, 36], [40, 60, 0]]
+    s.write(b, [0, 2, 0], [0, 60, 0])
+    t.release(0)                                                      # the last holder may write again
+    s.write(b, [0, 30, 0], [0, 30, 0])
+
+
+def test_steps_that_only_attend_may_stand_on_shared_pages(pkg, no_device):
+    t = no_device.PageTables(12, 16, 2, 96)
+    t.reserve(0, 48)
+    assert t.share(0, 1, 48) == 48
+    s, b = no_device.PagedStep(None, t, rows=4, max_rows=4, max_length=96), Written()
+    cache = no_device.PagedKvCache.__new__(no_device.PagedKvCache)
+    cache.kv_heads, cache.dim, cache.dtype, cache.pages, cache.page, cache.keys, cache.values = 1, 64, 2, 12, 16, None, None
+
+    class Kernels:
+        calls = 0
+
+        def paged_append_into(self, *a, **k):
+            Kernels.calls += 1
+    with pytest.raises(pkg.InvalidArgument):
+        s.write(b, [0, 1], [48, 48])
+    s.write(b, [0, 1], [48, 48], append=False)                        # a given beginning's last row once more, for its logits
+    assert b.all[-1].tolist() == [48, 48]
+    with pytest.raises(pkg.InvalidArgument, match="append"):
+        cache.append_into(None, Kernels(), s, None, None)
+    assert Kernels.calls == 0
+    t.reserve(1, 49)
+    s.write(b, [0, 1], [48, 49])
+    cache.append_into(None, Kernels(), s, None, None)
+    assert Kernels.calls == 1
