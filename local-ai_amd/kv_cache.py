@@ -325,6 +325,8 @@ class PageTables:
 
     def reserve(self, sequence: int, positions: int) -> None:
         """Pages for the sequence's first `positions` positions; all of what lacks or, where the pool has too few, nothing."""
+        if positions < 0:
+            raise InvalidArgument(f"{positions} positions")
         need = -(-positions // self.page)
         if need > self.table.shape[1]:
             raise InvalidArgument(f"{positions} positions in a table of {self.table.shape[1]} pages of {self.page}")
@@ -339,6 +341,8 @@ class PageTables:
     def share(self, source: int, target: int, positions: int) -> int:
         """Gives an empty sequence the whole pages of the source's first `positions` positions; returns how many positions those hold.  What
         stands there must be written already: neither sequence may append to them (``PagedStep.write`` refuses it)."""
+        if positions < 0:
+            raise InvalidArgument(f"{positions} positions")
         if self.held[target]:
             raise InvalidArgument(f"sequence {target} has pages")
         n = min(positions // self.page, self.held[source])

@@ -346,3 +346,17 @@ def test_steps_that_only_attend_may_stand_on_shared_pages(pkg, no_device):
     s.write(b, [0, 1], [48, 49])
     cache.append_into(None, Kernels(), s, None, None)
     assert Kernels.calls == 1
+
+
+def test_shares_of_fewer_than_no_positions_are_refused(pkg, no_device):
+    t = no_device.PageTables(12, 16, 3, 96)
+    t.reserve(0, 40)
+    for positions in (-1, -16, -17, -100):
+        with pytest.raises(pkg.InvalidArgument):
+            t.share(0, 1, positions)
+        with pytest.raises(pkg.InvalidArgument):
+            t.reserve(1, positions)
+    assert t.held == [3, 0, 0] and np.all(t.table[1] == t.NO_PAGE) and int(t.holders.sum()) == 3 and len(t.free) == 9
+    assert t.share(0, 1, 0) == 0
+    t.reserve(1, 0)
+    assert t.held[1] == 0
