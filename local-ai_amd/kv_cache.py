@@ -412,11 +412,16 @@ class PagedKvCache:
         nbytes = pages * kv_heads * page * kernels.paged_padded_dim(dim) * (4 if dtype == F32 else 2)
         self.keys, self.values = Buffer.empty(ctx, nbytes), Buffer.empty(ctx, nbytes)
 
+    def _check(self, step: PagedStep) -> None:
+        if step.tables.page != self.page or len(step.tables.holders) > self.pages:
+            raise InvalidArgument(f"tables of {len(step.tables.holders)} pages of {step.tables.page} positions for a cache of {self.pages} of {self.page}")
+
     def append_into(self, batch, kernels: Kernels, step: PagedStep, k: Buffer, v: Buffer, k_ld: int = 0, v_ld: int = 0,
                     rotary: Optional[Rotary] = None, q: Optional[Buffer] = None, q_output: Optional[Buffer] = None, heads: int = 0, q_ld: int = 0,
                     q_output_ld: int = 0) -> None:
         """The step's keys, turned, and values to their pages; its queries turned into `q_output` (may be `q`).  Rows without a distance lie
         one behind the other."""
+        self._check(step)
         if not step.appends:
             raise InvalidArgument("the step was written without append")
         n, h = self.kv_heads * self.dim, heads * self.dim
@@ -430,6 +435,7 @@ class PagedKvCache:
 
     def attention_into(self, batch, kernels: Kernels, step: PagedStep, q: Buffer, output: Buffer, heads: int, scale: float,
                        workspace: Optional[Buffer] = None, window: int = 0, sink: Optional[Buffer] = None, q_ld: int = 0, output_ld: int = 0) -> None:
+        self._check(step)
         h = heads * self.dim
         kernels.paged_attention_into(batch, q, self.keys, self.values, output, self.dtype, step.table, step.starts, step.lengths, step.rows,
                                      step.sequences, step.max_rows, step.max_length, heads, self.kv_heads, self.dim, self.pages, self.page,

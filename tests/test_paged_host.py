@@ -360,3 +360,28 @@ def test_shares_of_fewer_than_no_positions_are_refused(pkg, no_device):
     assert t.share(0, 1, 0) == 0
     t.reserve(1, 0)
     assert t.held[1] == 0
+
+
+def test_steps_of_other_pools_are_refused(pkg, no_device):
+    """Tables of another page size, or of more pages than the cache has, would send rows to wrong slots or drop them."""
+    class Kernels:
+        calls = 0
+
+        def paged_padded_dim(self, dim):
+            return padded(dim)
+
+        def paged_append_into(self, *a, **k):
+            Kernels.calls += 1
+        paged_attention_into = paged_append_into
+    K = Kernels()
+    for pages, page, right in ((12, 16, True), (12, 32, False), (6, 32, False), (13, 16, False), (11, 16, True)):
+        cache = no_device.PagedKvCache(None, K, 2, 64, 12, 16)
+        t = no_device.PageTables(pages, page, 2, 64)
+        s, before = no_device.PagedStep(None, t, 4, 4, 64), Kernels.calls
+        for call in (lambda: cache.append_into(None, K, s, None, None), lambda: cache.attention_into(None, K, s, None, None, 4, 0.1)):
+            if right:
+                call()
+            else:
+                with pytest.raises(pkg.InvalidArgument, match="pages"):
+                    call()
+        assert Kernels.calls - before == (2 if right else 0)
