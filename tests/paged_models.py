@@ -131,3 +131,17 @@ def attended(step, q, keys, values, scale, window=0, sink=None, max_length=None,
             off = (d + 8) * 2.0 ** -24 * size + 2.0 ** -22 * torch.maximum(z.abs().amax(1), top[:, 0].abs()) + 2.0 ** -21 + rounding + len(z[0]) * 2.0 ** -24
             tol[row] = torch.einsum("hp,phd->hd", w, vv.abs()) * 2 * off[:, None]
     return out, tol
+
+
+def told_apart(step, q, keys, values, scale, dtype, **more):
+    """Of outputs that are wrong in some way, the share of values that attention's tolerance tells from the right ones: zeros, negated ones, those of the pages one
+    further in the table, those of keys one slot further."""
+    want, tol = attended(step, q, keys, values, scale, **more)
+    tol = half_step(dtype) * want.abs() + tol + (2.0 ** -25 if dtype == "f16" else 0)
+    seen = tol > 0
+    other = Step.__new__(Step)
+    other.__dict__.update(step.__dict__)
+    other.table = np.stack([np.concatenate([np.roll(row[row != NO_PAGE], 1), row[row == NO_PAGE]]) for row in step.table]).astype(np.uint32)
+    wrong = {"zeros": torch.zeros_like(want), "negated": -want, "pages": attended(other, q, keys, values, scale, **more)[0],
+             "slots": attended(step, q, keys.roll(1, 2), values, scale, **more)[0]}
+    return {name: float(((w - want).abs() > tol)[seen].double().mean()) for name, w in wrong.items()}

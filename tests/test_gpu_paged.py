@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from paged_models import F64, NO_PAGE, TYPES, Step, appended, attended, half_step, padded, turn, turn_tolerance
+from paged_models import F64, NO_PAGE, TYPES, Step, appended, attended, half_step, padded, told_apart, turn, turn_tolerance
 
 pytestmark = pytest.mark.gpu
 BITS = {"f16": torch.int16, "bf16": torch.int16, "f32": torch.int32}
@@ -674,3 +674,74 @@ def test_what_is_read_may_stand_between_the_rows_of_an_output(dev):
     want, sizes = turn(x.reshape(rows, 1, 64), at, f, 1.0, 64, 0, True)
     close(got[:, :64].reshape(rows, 1, 64), want, turn_tolerance(want, sizes, "f32"))
     assert same_bits(got[:, 64:], whole[:, 64:], "f32")
+
+
+# ---- as they are used, from what is stored ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_session_against_what_its_pages_hold(dev, dtype):
+    """Prompts in chunks, tokens beside them, a shared beginning, sequences that end and whose pages serve the next.  The turned queries and the pages are read back:
+    keys and queries against 64 bits by the tolerance of a turn, outputs against attention over what stands there, by its own."""
+    from local_ai_amd import kv_cache as kv
+    pkg, K = dev.pkg, dev.K
+    H, G, dim, page, S, rows = 8, 2, 64, 16, 3, 90
+    tables = kv.PageTables(14, page, S, 160)
+    cache = kv.PagedKvCache(dev.ctx, K, G, dim, 14, page, code(pkg, dtype))
+    step = kv.PagedStep(dev.ctx, tables, rows, 64, 160)
+    f, _ = K.rotary_frequencies(dim, 1e4)
+    rotary = kv.Rotary(dev.up(f), dim)
+    work = pkg.Buffer.empty(dev.ctx, max(cache.workspace_bytes(K, step, H), 16))
+    told = [[] for _ in range(S)]                                   # (k, v) of every position
+    size = 4 if dtype == "f32" else 2
+
+    def run(counts, seed):
+        lengths = [len(t) + n for t, n in zip(told, counts)]
+        for s, (n, length) in enumerate(zip(counts, lengths)):
+            if n:
+                tables.reserve(s, length)
+        x = normal(seed, rows, (H + 2 * G) * dim, dtype=dtype)
+        qkv, out, batch = dev.up(x), pkg.Buffer.empty(dev.ctx, rows * H * dim * size), dev.batch()
+        step.write(batch, counts, lengths)
+        q, k, v = (qkv.view(o * dim * size, qkv.length() - o * dim * size) for o in (0, H, H + G))
+        ld = x.shape[1]
+        cache.append_into(batch, K, step, k, v, ld, ld, rotary, q, q, H, ld, ld)
+        cache.attention_into(batch, K, step, q, out, H, dim ** -0.5, work, q_ld=ld)
+        batch.commit_and_wait()
+        keys, values = (dev.down(b, (14, G, page, dim), dtype) for b in (cache.keys, cache.values))
+        heads = x.reshape(rows, H + 2 * G, dim)
+        turned = dev.down(qkv, (rows, H + 2 * G, dim), dtype)[:, :H]
+        model = Step([(n, length) for n, length in zip(counts, lengths)], page)
+        model.pages, model.table = 14, tables.table.copy()
+        places = list(model.places())
+        want, sizes = turn(heads[[p[0] for p in places], :H], [p[2] for p in places], f, 1.0, dim, 0, True)
+        close(turned[[p[0] for p in places]], want, turn_tolerance(want, sizes, dtype), "queries")
+        for s, n in enumerate(counts):
+            told[s] += [(heads[int(model.starts[s]) + i, H:H + G], heads[int(model.starts[s]) + i, H + G:]) for i in range(n)]
+        for s, length in enumerate(lengths):                        # all positions of all sequences, also of those that take no part
+            if length == 0:
+                continue
+            at = torch.arange(length)
+            pg = torch.as_tensor(tables.table[s].astype(np.int64))[at // page]
+            ks, vs = (torch.stack([t[i] for t in told[s]]) for i in range(2))
+            want, sizes = turn(ks, np.arange(length), f, 1.0, dim, 0, True)
+            close(keys[pg, :, at % page], want, turn_tolerance(want, sizes, dtype), "keys")
+            assert same_bits(values[pg, :, at % page], vs, dtype)
+        keys[~keys.isfinite()], values[~values.isfinite()] = 0, 0    # (slots that nobody has written)
+        want, tol = attended(model, turned[:model.rows], keys, values, dim ** -0.5)
+        close(dev.down(out, (rows, H, dim), dtype)[:model.rows], want, half_step(dtype) * want.abs() + tol + (2.0 ** -25 if dtype == "f16" else 0), counts)
+        apart = told_apart(model, turned[:model.rows], keys, values, dim ** -0.5, dtype)
+        assert min(apart[n] for n in ("zeros", "negated")) > 0.9, apart
+
+    run([40, 0, 0], 1)
+    run([24, 64, 0], 2)
+    run([1, 1, 0], 3)
+    shared = tables.share(0, 2, len(told[0]))
+    assert shared == 64
+    told[2] = told[0][:shared]
+    run([1, 1, 5], 4)
+    run([0, 1, 1], 5)
+    tables.release(1)
+    told[1] = []
+    run([1, 33, 1], 6)
+    tables.release(0)
+    told[0] = []
+    run([17, 1, 20], 7)

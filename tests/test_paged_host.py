@@ -5,8 +5,9 @@ import math
 
 import numpy as np
 import pytest
+import torch
 
-from paged_models import padded
+from paged_models import TYPES, Step, padded, told_apart
 
 
 # ---- frequencies ------------------------------------------------------------------------------------------------------------
@@ -385,3 +386,15 @@ def test_steps_of_other_pools_are_refused(pkg, no_device):
                 with pytest.raises(pkg.InvalidArgument, match="pages"):
                     call()
         assert Kernels.calls - before == (2 if right else 0)
+
+
+# ---- the tolerance -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sequences", [[(40, 40)], [(24, 64), (64, 64)], [(1, 65), (1, 65)], [(1, 67), (1, 66), (5, 69)]])
+def test_the_tolerance_of_attention_tells_wrong_results(dtype, sequences):
+    """The steps of a session of 8 heads of 64 over 2: outputs that are zero, negated, of other pages or other slots are not within it."""
+    step, g = Step(sequences, 16, seed=1), torch.Generator().manual_seed(2)
+    q = torch.randn(step.rows, 8, 64, generator=g).to(TYPES[dtype])
+    keys, values = (torch.randn(step.pages, 2, 16, 64, generator=g).to(TYPES[dtype]) for _ in range(2))
+    shares = told_apart(step, q, keys, values, 0.125, dtype)
+    assert min(shares.values()) > 0.9, shares
