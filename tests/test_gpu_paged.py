@@ -745,3 +745,35 @@ def test_a_session_against_what_its_pages_hold(dev, dtype):
     tables.release(0)
     told[0] = []
     run([17, 1, 20], 7)
+
+
+# ---- weights in two terms ------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,length", [(1, 65), (4, 65), (1, 600)])
+def test_weights_of_few_rows_have_two_terms(dev, dtype, rows, length):
+    """One position of weight 1 beside many of a weight that lies between two 16-bit numbers, whose values cancel, so that the output's own rounding hides nothing.
+
+    Rounded once, a weight is off by 0.49 of a step; what is left of it behind two terms is half a step of half a step, half_step^2.  The scores are 0 and ln w, a product
+    of one value by the scale: off by 2^-23 |ln w|, 2^-21 for the power of two; the sums of n weights and products n 2^-24 each; each of numerator and denominator."""
+    G, dim, H = 2, 64, 8 // rows
+    eps, half = torch.finfo(TYPES[dtype]).eps, half_step(dtype)
+    w = 0.5 * (1 + 0.49 * eps)
+    scale = float(np.float32(-math.log(w)))
+    step = Step([(rows, length)], 32, seed=length)
+    shape = (step.pages, G, 32, dim)
+    keys, values = torch.zeros(shape, dtype=TYPES[dtype]), torch.ones(shape, dtype=TYPES[dtype])
+    keys[..., 0] = -1.0
+    first = int(step.table[0, 0])
+    keys[first, :, 0, 0] = 0.0
+    values[first, :, 0] = -w * (length - 1)
+    q = torch.zeros(rows, H, dim, dtype=TYPES[dtype])
+    q[..., 0] = 1.0
+    want, _ = attended(step, q, keys, values, scale)
+    n = torch.arange(length - rows, length, dtype=F64)[:, None, None]              # positions of weight w that a row sees
+    big = values[first, 0, 0, 0].to(F64).abs()
+    off = 2.0 ** -23 + 2.0 ** -21 + (n + 1) * 2.0 ** -24 + (half ** 2 if dtype != "f32" else 0)
+    tol = half * want.abs() + 2 * off * (n * w + big) / (1 + n * w)
+    if dtype != "f32":                                              # one term would not be within it
+        once = (n * torch.tensor(w).to(TYPES[dtype]).to(F64) - big) / (1 + n * w)
+        assert bool(((once - want).abs() > 2 * tol).all())
+    close(attention_of(dev, step, q, keys, values, dtype, scale), want, tol)
