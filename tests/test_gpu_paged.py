@@ -747,7 +747,7 @@ def test_a_session_against_what_its_pages_hold(dev, dtype):
     run([17, 1, 20], 7)
 
 
-# ---- weights in two terms ------------------------------------------------------------------------------
+# ---- weights in two terms, and bounds beyond all sums ------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,length", [(1, 65), (4, 65), (1, 600)])
 def test_weights_of_few_rows_have_two_terms(dev, dtype, rows, length):
@@ -777,3 +777,12 @@ def test_weights_of_few_rows_have_two_terms(dev, dtype, rows, length):
         once = (n * torch.tensor(w).to(TYPES[dtype]).to(F64) - big) / (1 + n * w)
         assert bool(((once - want).abs() > 2 * tol).all())
     close(attention_of(dev, step, q, keys, values, dtype, scale), want, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,window", [(1, 0), (60, 0), (1, 700)])
+@pytest.mark.parametrize("bound", [0x7FFFFFFF, 0xFFFFFFFF])
+def test_attention_of_bounds_whose_steps_exceed_32_bits(dev, dtype, rows, window, bound):
+    """A call for lengths up to what a word holds, with so many tiles that what all have to do is summed in larger units."""
+    step = Step([(rows, 3000)] + [(rows, 60 + i) for i in range(70)] + [(1, 1500)], 64, seed=rows)
+    run_attention(dev, step, dtype, 8, 2, 64, window, seed=rows, max_length=bound)
