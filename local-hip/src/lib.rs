@@ -130,6 +130,41 @@ pub fn matmul_nt_qkv_attention_lanes_into(batch: &mut CommandBatch, fmt: ffi::lh
     })
 }
 
+/// `lh_paged_append_into` (include/local_hip.h) as `Kernels::paged_append_into` has it, and without rotation (`rot` 0) or without queries
+/// (`heads` 0).
+#[allow(clippy::too_many_arguments)]
+pub fn paged_append_into(batch: &mut CommandBatch, k: &Buffer, v: &Buffer, dtype: core::ffi::c_int, keys: &Buffer,
+                         values: &Buffer, table: &Buffer, starts: &Buffer, lengths: &Buffer, rows: u32, sequences: u32,
+                         kv_heads: u32, dim: u32, pages: u32, page: u32, table_ld: u32, k_ld: u32, v_ld: u32,
+                         frequencies: Option<&Buffer>, amplitude: f32, rot: u32, first: u32, pairing: u32,
+                         q: Option<&Buffer>, q_output: Option<&Buffer>, heads: u32, q_ld: u32,
+                         q_output_ld: u32) -> Result<()> {
+    // SAFETY: every pointer is null or comes from a live handle of this crate; the library validates sizes and shapes.
+    error::check(unsafe {
+        ffi::lh_paged_append_into(batch.as_ptr(), k.as_ptr(), v.as_ptr(), dtype, keys.as_ptr(), values.as_ptr(),
+                                  table.as_ptr(), starts.as_ptr(), lengths.as_ptr(), rows, sequences, kv_heads, dim,
+                                  pages, page, table_ld, k_ld, v_ld, opt(frequencies), amplitude, rot, first, pairing,
+                                  opt(q), opt(q_output), heads, q_ld, q_output_ld)
+    })
+}
+
+/// `lh_paged_attention_into` (include/local_hip.h) as `Kernels::paged_attention_into` has it, and for layers without sinks, and without a
+/// workspace where `lh_paged_attention_workspace_bytes` is 0.
+#[allow(clippy::too_many_arguments)]
+pub fn paged_attention_into(batch: &mut CommandBatch, q: &Buffer, keys: &Buffer, values: &Buffer, output: &Buffer,
+                            dtype: core::ffi::c_int, table: &Buffer, starts: &Buffer, lengths: &Buffer, rows: u32,
+                            sequences: u32, max_rows: u32, max_length: u32, heads: u32, kv_heads: u32, dim: u32,
+                            pages: u32, page: u32, table_ld: u32, q_ld: u32, output_ld: u32, scale: f32, window: u32,
+                            sink: Option<&Buffer>, workspace: Option<&Buffer>) -> Result<()> {
+    // SAFETY: every pointer is null or comes from a live handle of this crate; the library validates sizes and shapes.
+    error::check(unsafe {
+        ffi::lh_paged_attention_into(batch.as_ptr(), q.as_ptr(), keys.as_ptr(), values.as_ptr(), output.as_ptr(), dtype,
+                                     table.as_ptr(), starts.as_ptr(), lengths.as_ptr(), rows, sequences, max_rows,
+                                     max_length, heads, kv_heads, dim, pages, page, table_ld, q_ld, output_ld, scale,
+                                     window, opt(sink), opt(workspace))
+    })
+}
+
 /// `lh_matvec_quant_norm_chain_gelu_into` (include/local_hip.h): gate and up projection (or, with `factor` instead of `up`, one
 /// projection) behind a chain of norms, and the GeGLU product of their results where the launch can form it (layer.rs:476-482,
 /// 495-500).  `Ok(true)`: `out` holds the product.  `Ok(false)`: `out` and `up_out` hold the projections' results.

@@ -192,6 +192,26 @@ def test_steps_that_a_shared_cache_takes_without_keys_and_values():
                 assert (pname, arg) == (cname, cname), (name, cname)
 
 
+def test_paged_steps_without_what_the_header_lets_go():
+    """Models without sinks, calls without a workspace, appends without queries or rotation: lib.rs has both calls with the header's parameters in its order, the ones that
+    may be null as options."""
+    lib = open(os.path.join(ROOT, "local-hip", "src", "lib.rs")).read()
+    header = {f[0]: f for f in c_functions()}
+    for name, null in (("lh_paged_append_into", {"frequencies", "q", "q_output"}), ("lh_paged_attention_into", {"sink", "workspace"})):
+        sig, = re.findall(rf"pub fn {name[3:]}\(([^)]*)\) -> Result<\(\)>", lib)
+        params = [tuple(s.strip() for s in prm.split(":", 1)) for prm in sig.split(",")]
+        call, = re.findall(rf"ffi::{name}\(((?:[^()]|\([^()]*\))*)\)", lib)
+        args = [" ".join(a.split()) for a in call.split(",")]
+        cparams = header[name][2]
+        assert len(args) == len(params) == len(cparams)
+        for (ctype, cname), (pname, ptype), arg in zip(cparams, params, args):
+            if "lh_buffer" in ctype:
+                assert (pname, ptype) == (cname, "Option<&Buffer>" if cname in null else "&Buffer"), (name, cname)
+                assert arg == (f"opt({cname})" if cname in null else f"{cname}.as_ptr()"), (name, cname)
+            elif ctype != "lh_batch*":
+                assert (pname, ptype, arg) == (cname, SAFE_TYPES[ctype] if ctype != "int" else "core::ffi::c_int", cname), (name, cname)
+
+
 def test_safe_layer_argument_order_of_the_reference():
     """Three methods whose parameter lists were read off the reference (local-metal/src/kernels.rs:4819-4834, 5176-5193,
     5434-5452; kept here as data): the generated methods take exactly these parameters in exactly this order."""
