@@ -1105,7 +1105,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     int r = paged_check(op, keys, values, table, starts, lengths, dtype, sequences, kv_heads, dim, pages, page, table_ld);
     if (r != LH_OK) return r;
     LH_REQUIRE(heads > 0 && heads <= 65536 && heads % kv_heads == 0, "%s: heads %u is not a multiple of kv_heads %u", op, heads, kv_heads);
-    LH_REQUIRE(std::isfinite(scale), "%s: scale %g", op, (double)scale);
+    LH_REQUIRE(std::isfinite(scale * kLog2e), "%s: scale %g", op, (double)scale);      // (as the kernels have it)
     if (rows == 0) return LH_OK;
     LH_REQUIRE(max_rows > 0 && max_rows <= rows, "%s: %u rows, at most %u of a sequence", op, rows, max_rows);
     LH_REQUIRE((uint64_t)rows * heads < 0x7FFFFFFFull, "%s: %u rows of %u heads", op, rows, heads);

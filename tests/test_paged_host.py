@@ -398,3 +398,14 @@ def test_the_tolerance_of_attention_tells_wrong_results(dtype, sequences):
     keys, values = (torch.randn(step.pages, 2, 16, 64, generator=g).to(TYPES[dtype]) for _ in range(2))
     shares = told_apart(step, q, keys, values, 0.125, dtype)
     assert min(shares.values()) > 0.9, shares
+
+
+def test_scales_that_are_not_finite_in_powers_of_two_are_refused(pkg):
+    """Scores are kept in powers of two: a scale above the largest f32 over log2(e) would be an infinity there, and 0 times it NaN."""
+    pool = 2000 * 2 * 16 * 128 * 2
+    c = Call(pkg, "lh_paged_attention_into", batch=True, q=buf(GB, 6 * 800 * 2), keys=buf(3 * GB, pool), values=buf(4 * GB, pool), output=buf(2 * GB, 6 * 800 * 2), dtype=2,
+             table=buf(5 * GB, 3 * 1000 * 4), starts=buf(6 * GB, 16), lengths=buf(7 * GB, 12), rows=0, sequences=3, max_rows=4, max_length=16000, heads=8, kv_heads=2, dim=100,
+             pages=2000, page=16, table_ld=1000, q_ld=800, output_ld=800, scale=0.1, window=0, sink=buf(8 * GB, 32), workspace=None)
+    for scale in (3e38, -3e38, 2.36e38):
+        c.refused(scale=scale)
+    assert c.status(scale=2.35e38) == 0 and c.status(scale=-2.35e38) == 0
