@@ -954,9 +954,11 @@ LH_API int lh_rotary_rows_into(lh_batch* batch, const lh_buffer* input, lh_buffe
  *              one slot.
  *   attention  a row sees the positions up to its own, with `window` > 0 the last `window` of them; query heads share kv heads in equal
  *              groups.  out = softmax average with `scale`; sink f32 [heads] (may be null): exp(sink) is one more term of the denominator.
- *              A row that sees nothing becomes zero.  max_rows bounds a sequence's rows and max_length the lengths: they size the launch (a
- *              recorded batch gives the largest it will be replayed with); rows and positions beyond them are left out.  `workspace` takes
- *              lh_paged_attention_workspace_bytes (null where that is 0); its size goes by these arguments. */
+ *              A row that sees nothing becomes zero, and so does one all of whose scores are minus infinity.  Scores, sums and statistics are
+ *              of 32 bits; the weights that go into products of 16-bit types are two 16-bit terms where max_rows * heads / kv_heads is at
+ *              most 16, and are rounded once to 16 bits otherwise.  max_rows bounds a sequence's rows and max_length the lengths: they size
+ *              the launch (a recorded batch gives the largest it will be replayed with); rows and positions beyond them are left out.
+ *              `workspace` takes lh_paged_attention_workspace_bytes (null where that is 0); its size goes by these arguments. */
 LH_API uint32_t lh_paged_padded_dim(uint32_t dim);
 LH_API int lh_paged_append_into(lh_batch* batch, const lh_buffer* k, const lh_buffer* v, int dtype, lh_buffer* keys, lh_buffer* values,
                                 const lh_buffer* table, const lh_buffer* starts, const lh_buffer* lengths, uint32_t rows,

@@ -786,3 +786,30 @@ def test_attention_of_bounds_whose_steps_exceed_32_bits(dev, dtype, rows, window
     """A call for lengths up to what a word holds, with so many tiles that what all have to do is summed in larger units."""
     step = Step([(rows, 3000)] + [(rows, 60 + i) for i in range(70)] + [(1, 1500)], 64, seed=rows)
     run_attention(dev, step, dtype, 8, 2, 64, window, seed=rows, max_length=bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("length,max_length", [(100, 100), (6000, 6000), (300, 100000)])
+def test_positions_of_scores_of_minus_infinity_weigh_nothing(dev, dtype, rows, length, max_length):
+    """As what is masked; a row whose positions are all so becomes zero, as one that sees nothing."""
+    step = Step([(rows, length), (1, 50)], 32, seed=length)
+    shape = (step.pages, 2, 32, 64)
+    keys, values = normal(1, *shape, dtype=dtype), normal(2, *shape, dtype=dtype)
+    keys[..., 0] = 0.0
+    first = torch.from_numpy(step.table[0][step.table[0] != NO_PAGE].astype(np.int64))
+    keys[first, 1, :, 0] = -math.inf                               # all of the first sequence for one kv head, some positions for the other
+    keys[first, 0, ::3, 0] = -math.inf
+    q = normal(3, step.rows, 4, 64, dtype=dtype)
+    q[..., 0] = 1.0
+    got = attention_of(dev, step, q, keys, values, dtype, 0.125, max_length=max_length)
+    assert bool((got[:rows, 2:] == 0).all())
+    # the same without those positions: keys that score -2^9 there, whose weights 64 bits hold and 32 do not
+    low = keys.clone()
+    low[first, :, :, 0] = torch.where(keys[first, :, :, 0].isinf(), torch.tensor(-4096.0).to(TYPES[dtype]), keys[first, :, :, 0])
+    want, _ = attended(step, q, low, values, 0.125)
+    keys[first, :, :, 0] = torch.where(keys[first, :, :, 0].isinf(), torch.tensor(0.0).to(TYPES[dtype]), keys[first, :, :, 0])
+    _, tol = attended(step, q, keys, values, 0.125)
+    tol = half_step(dtype) * want.abs() + 2 * tol + (2.0 ** -25 if dtype == "f16" else 0)
+    close(got[:rows, :2], want[:rows, :2], tol[:rows, :2])
+    close(got[rows:], want[rows:], tol[rows:])
