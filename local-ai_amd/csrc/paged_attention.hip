@@ -1157,7 +1157,7 @@ int lh_paged_attention_into(lh_batch* batch, const lh_buffer* q, const lh_buffer
     if (dtype == LH_F32) r = launch_rows<kF32>(batch->ctx, a, c, tiles, op, launches);
     else if (dtype == LH_F16) r = launch_rows<kF16>(batch->ctx, a, c, tiles, op, launches);
     else r = launch_rows<kBf16>(batch->ctx, a, c, tiles, op, launches);
-    batch->dispatch_count += launches;
+    if (r == LH_OK) batch->dispatch_count += launches;
     return r;
 }
 
