@@ -91,7 +91,8 @@ __device__ __forceinline__ Load load_of(const PagedArgs& a, uint32_t s) {
 }
 
 // Steps of a part: what all tiles have to do over the workgroups wanted, so that a long sequence among short ones is cut and short ones alone are not, whatever bound the
-// call gives for their lengths (64 tokens at 4000 of a call for up to 131072: parts by the bound 313 us, so 171; 256 at 1000 653 and 174).  Where there are few tiles,
+// call gives for their lengths (64 tokens at 4000 of a call for up to 131072: parts by the bound 313 us, so 171; 256 at 1000 653 and 174).  The exception is a call whose
+// bounds fill the chip with tiles of at most 128 steps: nothing of it is cut (cut(), where it is measured).  Where there are few tiles,
 // equal ones make a whole number of parts.  It costs every workgroup two scans and a reciprocal, 0.2 us, and 5 with a thousand sequences (1024 at 1000 in a call for up to 16384
 // 658 -> 694 us).  All kernels of a call find the same.
 //   The sum is of steps shifted by `coarse` and rounded up, which lets it fit.  The chunk is at least what all have over `share`: so the parts of all tiles are at most
@@ -134,7 +135,7 @@ struct Tile {
 };
 // Part n of all tiles, JOIN: tile n of those in parts.  All lanes get the same; sequence -1 behind the last.  A sequence's tiles of the same part follow each other, so
 // that those that read the same pages at the same time are on different XCDs (on one, where the number of parts was a multiple of two, they waited for each
-// other: 64 rows at 8000 25.1 us, 20.4 so; 1000 rows of f32 54 and 44).
+// other: 64 rows at 8000 25.1 us, 20.4 so; 1000 rows of 8 heads over 4 of 128 in f32 54 and 44).
 template <uint32_t ROWS, uint32_t STEP, bool JOIN>
 __device__ __forceinline__ Tile tile_of(const PagedArgs& a, uint32_t n, uint32_t lane) {
     const uint32_t R = a.group.d;
@@ -299,7 +300,9 @@ template <int DT> constexpr float kLift = DT == kF16 ? 6.0f : 0.0f;
 
 // One packed row over positions begin .. end - 1, by one wave and value by value: what takes the place of the matrix instructions where a
 // result is not a number.  There a position that a row does not see has the weight 0, and 0 times an infinity or NaN that stands in it
-// is NaN; here it is left out.  Every lane gets the maximum (in powers of two) and the sum; sums[c] is of column lane + 64 c.
+// is NaN; here it is left out.  A wave takes all its rows so, whose positions
+// follow each other through the table, the key and the sum over lanes: one NaN among the values that all rows of a sequence see makes 64 tokens at 4096 to 16384 1610 us
+// instead of 430, 512 rows at position 16000 85 ms instead of 0.16.  Every lane gets the maximum (in powers of two) and the sum; sums[c] is of column lane + 64 c.
 template <int DT, int D>
 __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint64_t q_at, uint32_t g, uint32_t begin, uint32_t end, uint32_t lane,
                                                    float& m, float& l, float (&sums)[(D + 63) / 64]) {
@@ -342,6 +345,7 @@ __device__ __forceinline__ void slow_row(const PagedArgs& a, int sequence, uint6
 // stays that of its own rounding.
 // Memory binds it: 64 tokens over 4096 to 16384 positions of 8 kv heads of 128 (2.6 GB in pages of 16 positions, runs of 4 KB) 421 us, 6.2 TB/s,
 // where reading alone reaches 6.2 to 6.8 in runs of 8 KB; 15 % of a SIMD's time is vector and matrix work.  One token over 32768 (134 MB) 24 us.
+// 256 columns of 16 bits take 256 registers and keep two values in scratch (12 bytes a lane); f32 of 192 and 256 takes 272 and 324, one wave a SIMD.
 // The next step's keys are requested when this one's are used, its values likewise (the 64 tokens 450 -> 444 us).
 // The hint that nothing is read again, for caches that would push everything else out from near the chip: 472 -> 450, the token with its pages in memory
 // 31.9 -> 28.9 (where the last launch has left them near, 26.9 -> 27.3).  Pages that sequences share are read again, and soon: 64 tokens over the same 16384
@@ -610,9 +614,10 @@ __device__ __forceinline__ constexpr uint32_t key_place(uint32_t row) { return P
 //   O^T = V^T P^T  the weights are operands where they are; V, in LDS as it is in memory, is read by the transposing ds_read_b64_tr_b16
 // A weight is rounded once to 16 bits, which is what a result is off beside its own rounding: in bf16 0.0023 of it where that alone makes 0.0017.
 // (A second term as for few rows would be half as many products again.)
-// Issue binds it: 512 rows at position 16000 of 32 heads over 8 kv heads of 128 take 136 us, 1.0 PFLOP/s, at the 2.0 GHz that the chip keeps
-// there; the matrix instructions fill 47 % of a SIMD's time and the vector ones, which add to it, another 30; no bank conflicts.  Four prompts of 2048
-// to 4096 rows of 16 heads over 4: 206 us, 0.91.  The wave's priority is raised for the products (prompts 233 -> 231), operands are a group ahead
+// Issue binds it most: 512 rows at position 16000 of 32 heads over 8 kv heads of 128 take 136 to 141 us (from card to card), 0.97 to 1.0 PFLOP/s, at the 2.0 GHz that
+// the chip keeps there; the matrix instructions fill 46 % of a SIMD's time and the vector ones, which add to it, another 30.  The rest, 24 %, is waits: a step's barrier
+// and its loads, and reads of LDS, which is busy for 23 % of the time (every wave reads all keys and values of a step for its 32 rows; no bank conflicts).  Four prompts of
+// 2048 to 4096 rows of 16 heads over 4: 206 to 221 us, 0.85 to 0.91.  The wave's priority is raised for the products (prompts 233 -> 231), operands are a group ahead
 // (chunk 157 -> 153.5), the buffers' places are constants of a loop of two steps (156 -> 153.5).  256 columns: a wave a SIMD, 2000 rows of 8 heads
 // over one 62 us, 0.53.
 // In LDS the 16-byte pieces of a row change places by the row's low bits, so that neither read meets itself in one of the 64 banks: of
@@ -1022,6 +1027,8 @@ Cut cut(uint32_t tile_rows, uint32_t step, uint32_t dim, uint32_t rows, uint32_t
     // 2000 rows 71 -> 63; else two), parts of 256 (3 times 256 rows of 256 columns
     // and 29 tokens under a window of 512 27.5 us; 320 30.4).  Where the tiles alone fill
     // the chip and none is longer than 128 steps, none is cut: there is no second launch (four prompts of up to 4096 rows 225 -> 219 us, 256 tokens at 1000 178 -> 167).
+    // That goes by the call's bounds.  A step recorded for 256 tokens at up to 4096 that brings one, at 4096, takes 42.5 us, where one recorded for up to 4097 takes 21.8;
+    // with all 256 there 307 and 315.
     c.fill = tile_rows == 16 ? 2048 : dim > 192 ? 256 : 512;
     c.share = std::max(c.fill / kv_heads, 1u);
     const uint64_t units = c.tiles * kv_heads;

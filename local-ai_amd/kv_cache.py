@@ -374,7 +374,9 @@ class PagedStep:
 
     def write(self, batch, counts: Sequence[int], lengths: Sequence[int], append: bool = True) -> None:
         """Sequence s brings counts[s] rows (0: it takes no part) and has lengths[s] positions with them.  Rows that will be appended may not
-        stand on pages that another sequence holds, too; without `append` the step is for attention alone, over what is there."""
+        stand on pages that another sequence holds, too; without `append` the step is for attention alone, over what is there (a recorded
+        append is replayed only behind steps with it).  The whole table goes to the device: 0.04 ms of the host for 8 KB, 0.14 for 64, and a larger
+        one waits for the stream (256 KB 0.22, 1 MB 0.54)."""
         if len(counts) != self.sequences or len(lengths) != self.sequences:
             raise InvalidArgument(f"{len(counts)} and {len(lengths)} sequences of {self.sequences}")
         page = self.tables.page
