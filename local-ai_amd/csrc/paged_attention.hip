@@ -1028,7 +1028,7 @@ Cut cut(uint32_t tile_rows, uint32_t step, uint32_t dim, uint32_t rows, uint32_t
     // and 29 tokens under a window of 512 27.5 us; 320 30.4).  Where the tiles alone fill
     // the chip and none is longer than 128 steps, none is cut: there is no second launch (four prompts of up to 4096 rows 225 -> 219 us, 256 tokens at 1000 178 -> 167).
     // That goes by the call's bounds.  A step recorded for 256 tokens at up to 4096 that brings one, at 4096, takes 42.5 us, where one recorded for up to 4097 takes 21.8;
-    // with all 256 there 307 and 315.
+    // with all 256 there, over the same pages, 307 and 315.
     c.fill = tile_rows == 16 ? 2048 : dim > 192 ? 256 : 512;
     c.share = std::max(c.fill / kv_heads, 1u);
     const uint64_t units = c.tiles * kv_heads;
